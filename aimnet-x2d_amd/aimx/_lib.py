@@ -152,6 +152,36 @@ class EmbeddingTables(ctypes.Structure):
     ]
 
 
+DTYPE_F32, DTYPE_BF16 = 0, 1  # AIMX_DTYPE_*
+
+
+class Dense(ctypes.Structure):
+    """AimxDense (include/aimx.h): a dense or gated product."""
+    _fields_ = [
+        ("M", c_i64), ("N", c_i64), ("K", c_i64),
+        ("halves", c_i32), ("act", c_i32), ("dtype", c_i32), ("precision", c_i32),
+        ("x", c_ptr), ("ldx", c_i64),
+        ("w", c_ptr * 2), ("ldw", c_i64),
+        ("b", c_ptr * 2),
+        ("res", c_ptr), ("ldr", c_i64),
+        ("y", c_ptr), ("ldy", c_i64),
+        ("pre", c_ptr),
+        ("q", c_ptr), ("qexp", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", c_size),
+    ]
+
+
+class DenseGrad(ctypes.Structure):
+    """AimxDenseGrad (include/aimx.h): the gradients of a dense or gated product."""
+    _fields_ = [
+        ("dy", c_ptr), ("ldd", c_i64),
+        ("dx", c_ptr), ("lddx", c_i64),
+        ("dw", c_ptr * 2),
+        ("db", c_ptr * 2),
+        ("workspace", c_ptr), ("workspace_bytes", c_size),
+    ]
+
+
 class CopyItem(ctypes.Structure):
     _fields_ = [("src", c_ptr), ("dst", c_ptr), ("n", c_i64)]
 
@@ -210,6 +240,12 @@ _SIGS = {
     "aimx_embedding_gather": (c_i32, [ctypes.POINTER(EmbeddingTables), c_i64, c_ptr, c_i64, c_ptr]),
     "aimx_embedding_backward_workspace_bytes": (c_size, [ctypes.POINTER(EmbeddingTables), c_i64]),
     "aimx_embedding_backward": (c_i32, [ctypes.POINTER(EmbeddingTables), c_i64, c_ptr, c_i64, c_ptr, c_size, c_ptr]),
+    "aimx_dense_workspace_bytes": (c_size, [ctypes.POINTER(Dense)]),
+    "aimx_dense_forward": (c_i32, [ctypes.POINTER(Dense), c_ptr]),
+    "aimx_dense_backward_workspace_bytes": (c_size, [ctypes.POINTER(Dense), ctypes.POINTER(DenseGrad)]),
+    "aimx_dense_backward": (c_i32, [ctypes.POINTER(Dense), ctypes.POINTER(DenseGrad), c_ptr]),
+    "aimx_pack8": (c_i32, [c_i32, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
+    "aimx_unpack8": (c_i32, [c_i32, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_ptr]),
     "aimx_act_backward": (c_i32, [c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr]),
     "aimx_act_backward2": (c_i32, [c_i32, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64,
                                    c_ptr]),

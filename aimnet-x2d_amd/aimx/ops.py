@@ -1132,3 +1132,249 @@ def head(x_pooled, wp, bp, blocks, ws, bs, wo, bo, *, act, drop_p=0.0, training=
     for b in blocks:
         flat += list(b)
     return _Head.apply(spec, seed if drop else None, x_pooled, wp, bp, *flat, ws, bs, wo, bo)
+
+
+# ---------------------------------------------------------------------------------------------
+# Dense and gated products on 32- and 16-bit tensors, with 8-bit activation checkpoints
+# (csrc/dense.hip, csrc/pack8.hip)
+# ---------------------------------------------------------------------------------------------
+_DTYPES = {_F32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+PACK8_GROUP = 32
+
+
+class _on:
+    """Makes `device` the current one for the kernels launched inside, if it is not already."""
+
+    def __init__(self, device):
+        self.device, self.back = device, None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if self.device.index is not None and self.device.index != now:
+            self.back = now
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+        return False
+
+
+def _matrix(what, name, t):
+    """(t as [M, K] rows, row stride); t has unit column stride or is copied."""
+    t, ld = _rows(t.reshape(-1, t.shape[-1]))
+    if ld > 1 << 21:
+        raise _lib.AimxError(f"aimx.{what}: {name} has a row stride over 2^21 elements")
+    return t, ld
+
+
+class Packed8:
+    """A tensor held in 8 bits (pack8): q int8 [M, Kq], exps int8 [M, Kq / 32], the shape and dtype it had.
+    nbytes is 33/32 of a byte per value (rows padded to 32)."""
+    __slots__ = ("q", "exps", "shape", "dtype")
+
+    def __init__(self, q, exps, shape, dtype):
+        self.q, self.exps, self.shape, self.dtype = q, exps, shape, dtype
+
+    @property
+    def nbytes(self):
+        return self.q.numel() + self.exps.numel()
+
+
+def _pack8(what, x):
+    if x.dtype not in _DTYPES:
+        raise _lib.AimxError(f"aimx.{what}: fp32 or bf16 tensors, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise _lib.AimxError(f"aimx.{what}: the last dimension must hold at least one value")
+    x2, ld = _rows(x.reshape(-1, x.shape[-1]))
+    M, K = x2.shape
+    kq = -(-K // PACK8_GROUP) * PACK8_GROUP
+    q = torch.empty(M, kq, dtype=torch.int8, device=x.device)
+    exps = torch.empty(M, kq // PACK8_GROUP, dtype=torch.int8, device=x.device)
+    with _on(x.device):
+        check(_lib.load().aimx_pack8(_DTYPES[x.dtype], ptr(x2), ld, M, K, ptr(q), ptr(exps), stream_ptr(x.device)),
+              "pack8")
+    return Packed8(q, exps, tuple(x.shape), x.dtype)
+
+
+def pack8(x):
+    """The 8-bit form of a fp32 or bf16 tensor: groups of 32 values along the last dimension share a
+    power-of-two scale 2^e, the least (from 2^-126) with 127 * 2^e >= max|x|; values are rounded to nearest
+    even, so each comes back within 2^(e-1) <= max|x| / 127 of itself. A group with a NaN or an infinity comes
+    back as NaN. Not differentiable (checkpoint8=True of dense and gated_linear is)."""
+    _lib.require_device(x)
+    return _pack8("pack8", x.detach())
+
+
+def unpack8(packed, dtype=None):
+    """The values a Packed8 stands for, in its own dtype or `dtype` (exact in both fp32 and bf16)."""
+    dtype = packed.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise _lib.AimxError(f"aimx.unpack8: fp32 or bf16, got {dtype}")
+    dev, K = packed.q.device, packed.shape[-1]
+    out = torch.empty(packed.shape, dtype=dtype, device=dev)
+    with _on(dev):
+        check(_lib.load().aimx_unpack8(_DTYPES[dtype], ptr(packed.q), ptr(packed.exps), packed.q.shape[0], K, ptr(out),
+                                       K, stream_ptr(dev)), "unpack8")
+    return out
+
+
+def _dense_struct(x2, ldx, ws, bs, act, prec):
+    d = _lib.Dense()
+    w = ws[0]
+    d.M, d.N, d.K = x2.shape[0], w.shape[0], w.shape[1]
+    d.halves, d.act, d.dtype, d.precision = len(ws), act, _DTYPES[w.dtype], prec
+    d.x, d.ldx = ptr(x2), ldx
+    d.ldw = w.shape[1]
+    for i, (wi, bi) in enumerate(zip(ws, bs)):
+        d.w[i], d.b[i] = ptr(wi), ptr(bi)
+    return d
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _dense_forward(x, ws, bs, res, act, prec, keep_pre):
+    """(y, pre or None, x as rows): one forward on the current stream of x's device."""
+    import ctypes
+    lib = _lib.load()
+    dev = x.device
+    x2, ldx = _matrix("dense", "x", x)
+    n = ws[0].shape[0]
+    d = _dense_struct(x2, ldx, ws, bs, act, prec)
+    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
+    d.y, d.ldy = ptr(y), n
+    if res is not None:
+        r2, d.ldr = _matrix("dense", "residual", res)
+        d.res = ptr(r2)
+    pre = None
+    if keep_pre:
+        pre = torch.empty(d.M, len(ws) * n, dtype=_F32, device=dev)
+        d.pre = ptr(pre)
+    with _on(dev):
+        d.workspace_bytes = lib.aimx_dense_workspace_bytes(ctypes.byref(d))
+        work = _workspace(d.workspace_bytes, dev)
+        d.workspace = ptr(work)
+        check(lib.aimx_dense_forward(ctypes.byref(d), stream_ptr(dev)), "dense_forward")
+    return y, pre, x2
+
+
+class _DenseFn(torch.autograd.Function):
+    """halves = 1: dense(x, w, b, residual); halves = 2: gated_linear(x, w_gate, w_up, b_gate, b_up). Kept for
+    the backward: x (or its 8-bit form) and, unless checkpoint8, the fp32 values before the activation."""
+
+    @staticmethod
+    def forward(ctx, x, w0, w1, b0, b1, res, act, checkpoint8):
+        ws = [w0.contiguous()] + ([w1.contiguous()] if w1 is not None else [])
+        bs = [b.contiguous() if b is not None else None for b in ((b0, b1) if w1 is not None else (b0,))]
+        ctx.prec = amp_precision() if x.dtype == _F32 else PREC_FP32
+        need = ctx.needs_input_grad
+        y, pre, x2 = _dense_forward(x, ws, bs, res, act, ctx.prec, act >= 0 and not checkpoint8 and any(need[:5]))
+        ctx.act, ctx.shape, ctx.halves = act, x.shape, len(ws)
+        kept, exps = x2, None
+        if checkpoint8:
+            p = _pack8("dense", x2)
+            kept, exps = p.q, p.exps
+        ctx.save_for_backward(kept, exps, pre, *ws, *bs)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        import ctypes
+        lib = _lib.load()
+        kept, exps, pre, *rest = ctx.saved_tensors
+        ws, bs = rest[:ctx.halves], rest[ctx.halves:]
+        need = ctx.needs_input_grad
+        dev = dy.device
+        n, k = ws[0].shape
+        dy2, ldd = _matrix("dense", "dy", dy)
+        d = _dense_struct(kept, kept.stride(0), ws, bs, ctx.act, ctx.prec)
+        if exps is not None:
+            d.x, d.ldx, d.q, d.qexp = None, 0, ptr(kept), ptr(exps)
+        else:
+            d.ldx = max(kept.stride(0), k)  # a single row's stride is whatever it is
+        d.pre = ptr(pre)
+        g = _lib.DenseGrad()
+        g.dy, g.ldd = ptr(dy2), ldd
+        dx = dw = db = None
+        if need[0]:
+            dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dev)
+            g.dx, g.lddx = ptr(dx), k
+        if need[1] or need[2]:
+            dw = [torch.empty_like(w) for w in ws]
+            for i, t in enumerate(dw):
+                g.dw[i] = ptr(t)
+        if need[3] or need[4]:
+            db = [torch.empty(n, dtype=dy.dtype, device=dev) for _ in ws]
+            for i, t in enumerate(db):
+                g.db[i] = ptr(t)
+        if dx is not None or dw is not None or db is not None:
+            with _on(dev):
+                g.workspace_bytes = lib.aimx_dense_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(g))
+                work = _workspace(g.workspace_bytes, dev)
+                g.workspace = ptr(work)
+                check(lib.aimx_dense_backward(ctypes.byref(d), ctypes.byref(g), stream_ptr(dev)), "dense_backward")
+        at = lambda v, i: v[i] if v is not None and i < len(v) and need[i + (1 if v is dw else 3)] else None  # noqa: E731
+        return dx, at(dw, 0), at(dw, 1), at(db, 0), at(db, 1), dy if need[5] else None, None, None
+
+
+def _dense_checks(what, x, ws, bs, act, res=None):
+    _lib.require_device(x, *ws, *bs, res)
+    if x.dtype not in _DTYPES:
+        raise _lib.AimxError(f"aimx.{what}: fp32 or bf16 tensors, got {x.dtype}")
+    if x.dim() < 1 or any(w.dim() != 2 or w.shape != ws[0].shape for w in ws) or ws[0].shape[1] != x.shape[-1] or \
+            min(ws[0].shape) < 1:
+        raise _lib.AimxError(f"aimx.{what}: weights [n_out, n_in] for x [..., n_in], got "
+                             f"{[tuple(w.shape) for w in ws]} and {tuple(x.shape)}")
+    n = ws[0].shape[0]
+    if any(b is not None and b.shape != (n,) for b in bs):
+        raise _lib.AimxError(f"aimx.{what}: biases are [n_out]")
+    if res is not None and res.shape != (*x.shape[:-1], n):
+        raise _lib.AimxError(f"aimx.{what}: the residual has the result's shape {(*x.shape[:-1], n)}, got "
+                             f"{tuple(res.shape)}")
+    for t in (*ws, *bs, res):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise _lib.AimxError(f"aimx.{what}: every tensor has x's dtype and device ({x.dtype}, {x.device})")
+    if max(ws[0].shape) > 1 << 21:
+        raise _lib.AimxError(f"aimx.{what}: widths up to 2^21")
+    if act is None:
+        return -1
+    if act not in _lib.ACT_KIND:
+        raise _lib.AimxError(f"aimx.{what}: act is one of {', '.join(_lib.ACT_KIND)}")
+    return _lib.ACT_KIND[act]
+
+
+def _dense_apply(what, x, ws, bs, res, act, checkpoint8):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *ws, *bs, res)):
+        if x.numel() // x.shape[-1] > 1 << 22:
+            raise _lib.AimxError(f"aimx.{what}: at most 2^22 rows where gradients are asked for")
+        two = len(ws) == 2
+        return _DenseFn.apply(x, ws[0], ws[1] if two else None, bs[0], bs[1] if two else None, res, act,
+                              bool(checkpoint8))
+    prec = amp_precision() if x.dtype == _F32 else PREC_FP32
+    return _dense_forward(x, [w.contiguous() for w in ws], [b.contiguous() if b is not None else None for b in bs], res,
+                          act, prec, False)[0]
+
+
+def dense(x, w, b=None, act=None, residual=None, checkpoint8=False):
+    """y = act(x w^T + b) + residual in one kernel: x [..., n_in], w [n_out, n_in], b [n_out] or None, act None
+    or an activation name, residual [..., n_out] or None; all fp32 or all bf16. fp32 at fp32 accuracy
+    (bf16 operands inside torch.autocast, as linear()). Differentiable in every tensor.
+    checkpoint8=True: the backward keeps x in 8 bits (pack8: 33/32 bytes a value) instead of x and the
+    values before the activation, and computes the gradients for the x that those bits stand for."""
+    kind = _dense_checks("dense", x, [w], [b], act, residual)
+    return _dense_apply("dense", x, [w], [b], residual, kind, checkpoint8)
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", checkpoint8=False):
+    """h = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both projections, the activation and the product in one
+    kernel. x [..., n_in], weights [n_out, n_in], biases [n_out] or None (both or neither). Types, autocast
+    and checkpoint8 as in dense()."""
+    if act is None:
+        raise _lib.AimxError("aimx.gated_linear: act names the gate's activation")
+    if (b_gate is None) != (b_up is None):
+        raise _lib.AimxError("aimx.gated_linear: both biases or neither")
+    kind = _dense_checks("gated_linear", x, [w_gate, w_up], [b_gate, b_up], act)
+    return _dense_apply("gated_linear", x, [w_gate, w_up], [b_gate, b_up], None, kind, checkpoint8)

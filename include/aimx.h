@@ -581,6 +581,66 @@ typedef struct AimxPadBatch {
 int aimx_pad_batch(const AimxPadBatch* p, aimx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Dense and gated products (aimx.ops.dense / gated_linear), 32- and 16-bit tensors:
+ *   halves 1:  y = act(x W^T + b) + res          (act may be AIMX_ACT_NONE, b and res NULL)
+ *   halves 2:  y = act(x W0^T + b0) * (x W1^T + b1)   (one kernel; res must be NULL)
+ * x [M, K] (row stride ldx), each w [N, K] (row stride ldw), each b [N], res and y [M, N]: all of `dtype`.
+ * precision: of fp32 tensors. AIMX_PREC_FP32: fp32 accuracy on the bf16 matrix cores (three exact bf16
+ * parts per operand, six products); AIMX_PREC_BF16: operands rounded to bf16, everything else fp32.
+ * Sums are fp32. An infinite operand of an AIMX_PREC_FP32 product may give NaN instead of an infinity.
+ * pre (nullable, fp32 [M, halves * N], 16-byte aligned): the values before the activation, kept for
+ * aimx_dense_backward; without them (act != none) the backward computes them again.
+ * The workspace (16-byte aligned, aimx_dense_workspace_bytes / aimx_dense_backward_workspace_bytes) holds
+ * staged operands and partial sums. Sums over ranges of k and of rows are joined in a fixed order.
+ * Row strides <= 2^21 elements, N, K <= 2^21; the backward takes M <= 2^22 rows.
+ *
+ * aimx_dense_backward: dy [M, N] -> dx [M, K], dw [N, K] (contiguous), db [N], each written when its
+ * pointer is given (dw and db of both halves or of neither). It reads x, w, pre of d (b only where pre is
+ * NULL); with x NULL it runs on the 8-bit form of x (q, qexp: aimx_pack8), whose values it takes for x also
+ * where it computes pre again. bf16 tensors: the gradient before the activation is rounded to bf16 once.
+ * M = 0: dw and db are zero-filled.
+ * ------------------------------------------------------------------------------------------ */
+#define AIMX_DTYPE_F32 0
+#define AIMX_DTYPE_BF16 1
+typedef struct AimxDense {
+  int64_t M, N, K;
+  int32_t halves, act, dtype, precision;
+  const void* x; int64_t ldx;
+  const void* w[2]; int64_t ldw;
+  const void* b[2];
+  const void* res; int64_t ldr;
+  void* y; int64_t ldy;
+  float* pre;
+  const int8_t* q; const int8_t* qexp;
+  void* workspace; size_t workspace_bytes;
+} AimxDense;
+
+typedef struct AimxDenseGrad {
+  const void* dy; int64_t ldd;
+  void* dx; int64_t lddx;
+  void* dw[2];
+  void* db[2];
+  void* workspace; size_t workspace_bytes;
+} AimxDenseGrad;
+
+size_t aimx_dense_workspace_bytes(const AimxDense* d);
+int aimx_dense_forward(const AimxDense* d, aimx_stream_t stream);
+size_t aimx_dense_backward_workspace_bytes(const AimxDense* d, const AimxDenseGrad* g);
+int aimx_dense_backward(const AimxDense* d, const AimxDenseGrad* g, aimx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Activations in 8 bits (aimx.ops.pack8 / unpack8): groups of 32 values along a row share the scale
+ * 2^e, e the least integer >= -126 with 127 * 2^e >= max|x| of the group; q = round-to-even(x / 2^e).
+ * q [M, Kq] int8 (8-byte aligned, zeros behind column K), exps [M, Kq / 32] int8, Kq = K rounded up to 32.
+ * A group with a NaN or an infinity has e = 127 and unpacks as NaN. q * 2^e is exactly a bf16. The largest
+ * fp32 values (e = 122) are kept below overflow (|q| <= 63).
+ * ------------------------------------------------------------------------------------------ */
+int aimx_pack8(int32_t dtype, const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* q, int8_t* exps,
+               aimx_stream_t stream);
+int aimx_unpack8(int32_t dtype, const int8_t* q, const int8_t* exps, int64_t M, int64_t K, void* y, int64_t ldy,
+                 aimx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Gradient all-reduce over RCCL (xGMI inside an MI355X node) — the DDP reducer's collective
  * (reference runner.py:703-707 wraps the model in DistributedDataParallel over "nccl" = RCCL).
  * RCCL is resolved at run time (aimx_comm_load: dlopen of the RCCL the process already uses, e.g.
