@@ -246,6 +246,10 @@ _SIGS = {
     "aimx_dense_backward": (c_i32, [ctypes.POINTER(Dense), ctypes.POINTER(DenseGrad), c_ptr]),
     "aimx_pack8": (c_i32, [c_i32, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
     "aimx_unpack8": (c_i32, [c_i32, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_ptr]),
+    "aimx_token_embedding_forward": (c_i32, [c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_f32, c_ptr, c_ptr]),
+    "aimx_token_embedding_backward_workspace_bytes": (c_size, [c_i32, c_i64, c_i64, c_i64]),
+    "aimx_token_embedding_backward": (c_i32, [c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_f32, c_i64, c_ptr,
+                                              c_ptr, c_size, c_ptr]),
     "aimx_act_backward": (c_i32, [c_i32, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr]),
     "aimx_act_backward2": (c_i32, [c_i32, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64,
                                    c_ptr]),

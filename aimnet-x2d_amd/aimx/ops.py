@@ -8,6 +8,11 @@ Each operator corresponds to a reference interface:
   segment_pool           <- Mean/Max/SumPoolingLayer.forward (pooling.py:15-80)
   partial_charges        <- GNN._partial_charge_calculation (gnn.py:622-658)
   l1_loss                <- nn.L1Loss / WeightedL1Loss (trainer.py:24-35, models/losses.py:14-48)
+Beside the reference's own, for feed-forward stages on 32- and 16-bit tensors:
+  dense                  product with bias, activation and a residual behind it
+  gated_linear           both projections of a gated block, the activation and the product in one kernel
+  pack8 / unpack8        activations in 8 bits; checkpoint8=True of dense and gated_linear keeps them so
+  embedding              scaled lookup in a table of any size, gradient by sorted tokens
 """
 from __future__ import annotations
 
@@ -1186,6 +1191,7 @@ def _pack8(what, x):
         raise _lib.AimxError(f"aimx.{what}: fp32 or bf16 tensors, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise _lib.AimxError(f"aimx.{what}: the last dimension must hold at least one value")
+    _lib.require_device(x)
     x2, ld = _rows(x.reshape(-1, x.shape[-1]))
     M, K = x2.shape
     kq = -(-K // PACK8_GROUP) * PACK8_GROUP
@@ -1202,7 +1208,6 @@ def pack8(x):
     power-of-two scale 2^e, the least (from 2^-126) with 127 * 2^e >= max|x|; values are rounded to nearest
     even, so each comes back within 2^(e-1) <= max|x| / 127 of itself. A group with a NaN or an infinity comes
     back as NaN. Not differentiable (checkpoint8=True of dense and gated_linear is)."""
-    _lib.require_device(x)
     return _pack8("pack8", x.detach())
 
 
@@ -1321,7 +1326,6 @@ class _DenseFn(torch.autograd.Function):
 
 
 def _dense_checks(what, x, ws, bs, act, res=None):
-    _lib.require_device(x, *ws, *bs, res)
     if x.dtype not in _DTYPES:
         raise _lib.AimxError(f"aimx.{what}: fp32 or bf16 tensors, got {x.dtype}")
     if x.dim() < 1 or any(w.dim() != 2 or w.shape != ws[0].shape for w in ws) or ws[0].shape[1] != x.shape[-1] or \
@@ -1339,11 +1343,10 @@ def _dense_checks(what, x, ws, bs, act, res=None):
             raise _lib.AimxError(f"aimx.{what}: every tensor has x's dtype and device ({x.dtype}, {x.device})")
     if max(ws[0].shape) > 1 << 21:
         raise _lib.AimxError(f"aimx.{what}: widths up to 2^21")
-    if act is None:
-        return -1
-    if act not in _lib.ACT_KIND:
+    if act is not None and act not in _lib.ACT_KIND:
         raise _lib.AimxError(f"aimx.{what}: act is one of {', '.join(_lib.ACT_KIND)}")
-    return _lib.ACT_KIND[act]
+    _lib.require_device(x)
+    return -1 if act is None else _lib.ACT_KIND[act]
 
 
 def _dense_apply(what, x, ws, bs, res, act, checkpoint8):
@@ -1378,3 +1381,65 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", checkpoint
         raise _lib.AimxError("aimx.gated_linear: both biases or neither")
     kind = _dense_checks("gated_linear", x, [w_gate, w_up], [b_gate, b_up], act)
     return _dense_apply("gated_linear", x, [w_gate, w_up], [b_gate, b_up], None, kind, checkpoint8)
+
+
+# ---------------------------------------------------------------------------------------------
+# Scaled embedding with the gradient by sorted tokens (csrc/tokens.hip)
+# ---------------------------------------------------------------------------------------------
+def _embedding_forward(index, table, scale):
+    D = table.shape[1]
+    out = torch.empty(*index.shape, D, dtype=table.dtype, device=table.device)
+    with _on(table.device):
+        check(_lib.load().aimx_token_embedding_forward(_DTYPES[table.dtype], ptr(index), index.numel(), ptr(table),
+                                                       table.shape[0], D, scale, ptr(out), stream_ptr(table.device)),
+              "token_embedding_forward")
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, index, table, scale, padding_idx):
+        table = table.contiguous()
+        ctx.save_for_backward(index)
+        ctx.table, ctx.scale, ctx.padding_idx = (table.shape, table.dtype), scale, padding_idx
+        return _embedding_forward(index, table, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        lib = _lib.load()
+        index, = ctx.saved_tensors
+        (V, D), dtype = ctx.table
+        dev = dy.device
+        dy2, ldd = _rows(dy.reshape(-1, D))
+        grad = torch.empty(V, D, dtype=dtype, device=dev)
+        with _on(dev):
+            nbytes = lib.aimx_token_embedding_backward_workspace_bytes(_DTYPES[dtype], index.numel(), V, D)
+            work = _workspace(nbytes, dev)
+            check(lib.aimx_token_embedding_backward(_DTYPES[dtype], ptr(index), index.numel(), ptr(dy2), ldd, V, D,
+                                                    ctx.scale, ctx.padding_idx, ptr(grad), ptr(work), nbytes,
+                                                    stream_ptr(dev)), "token_embedding_backward")
+        return None, grad, None, None
+
+
+def embedding(index, table, scale=1.0, padding_idx=None):
+    """scale * table[index]: index an integer tensor of any shape, table [V, D] fp32 or bf16 of any size. The
+    gradient sums each token's rows in fp32 in ascending position (deterministic). An index outside
+    [0, V) gives a zero row and no gradient; padding_idx (negative: from the end) gets no gradient."""
+    if table.dim() != 2 or min(table.shape) < 1 or table.dtype not in _DTYPES:
+        raise _lib.AimxError("aimx.embedding: table [V, D] of fp32 or bf16")
+    if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
+        raise _lib.AimxError(f"aimx.embedding: integer indices, got {index.dtype}")
+    if index.device != table.device:
+        raise _lib.AimxError("aimx.embedding: index and table on one device")
+    V = table.shape[0]
+    if V >= 2 ** 31 - 1 or index.numel() >= 2 ** 31 - 1 or table.shape[1] > 1 << 24:
+        raise _lib.AimxError("aimx.embedding: at most 2^31 - 2 rows and indices, 2^24 columns")
+    if padding_idx is not None and not -V <= padding_idx < V:
+        raise _lib.AimxError(f"aimx.embedding: padding_idx in [-{V}, {V})")
+    pad = -1 if padding_idx is None else int(padding_idx) % V
+    _lib.require_device(table)
+    index = index.to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _Embedding.apply(index, table, float(scale), pad)
+    return _embedding_forward(index, table.contiguous(), float(scale))

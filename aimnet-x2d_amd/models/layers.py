@@ -168,3 +168,40 @@ class MultiLayerPerceptron(nn.Module):
         for layer in self.layers:
             x = layer(x)
         return x
+
+
+class GatedBlock(nn.Module):
+    """The gated form of LinearBlock: act(gate(x)) * up(x) -> down, with an identity skip where the widths
+    agree. Two kernels forward (ops.gated_linear; ops.dense with the skip in its epilogue); fp32 or bf16
+    parameters. checkpoint8=True keeps the inputs of both products in 8 bits for the backward instead of
+    themselves and the values before the activation (ops.pack8)."""
+
+    def __init__(self, input_dim: int, hidden_dim: int, output_dim: int, activation_type: str = "silu",
+                 use_skip: bool = True, bias: bool = True, checkpoint8: bool = False):
+        super().__init__()
+        self.use_skip = use_skip and (input_dim == output_dim)
+        self.checkpoint8 = checkpoint8
+        self.gate = nn.Linear(input_dim, hidden_dim, bias=bias)
+        self.up = nn.Linear(input_dim, hidden_dim, bias=bias)
+        self.activation = get_activation_function(activation_type)
+        self.down = nn.Linear(hidden_dim, output_dim, bias=bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        h = ops.gated_linear(x, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias,
+                             act=activation_name(self.activation), checkpoint8=self.checkpoint8)
+        return ops.dense(h, self.down.weight, self.down.bias, residual=x if self.use_skip else None,
+                         checkpoint8=self.checkpoint8)
+
+
+class ScaledEmbedding(nn.Embedding):
+    """nn.Embedding on ops.embedding: the rows times `scale` (an integer tensor of any shape in, table of any
+    size), the gradient summed in fp32 over the sorted tokens."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int = None, **kw):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, **kw)
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise ValueError("ScaledEmbedding: max_norm, scale_grad_by_freq and sparse are not supported")
+        self.scale = scale
+
+    def forward(self, index: torch.Tensor) -> torch.Tensor:
+        return ops.embedding(index, self.weight, self.scale, self.padding_idx)

@@ -641,6 +641,22 @@ int aimx_unpack8(int32_t dtype, const int8_t* q, const int8_t* exps, int64_t M, 
                  aimx_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Scaled embedding of one table of any size (aimx.ops.embedding; the small-table gather above takes several
+ * tables of at most 160 KB together):
+ *   forward   out[i] = scale * table[index[i]]                    out [n, D], table [V, D], contiguous
+ *   backward  dtable[v] = scale * sum over i with index[i] = v of dy[i], ascending i, in fp32 (deterministic:
+ *             tokens sorted by id, runs summed in order); every row of dtable [V, D] is written (16-byte aligned)
+ * An index outside [0, V) gives a zero row and no gradient; rows equal to padding_idx (-1: none) give no
+ * gradient. n, V < 2^31 - 1.
+ * ------------------------------------------------------------------------------------------ */
+int aimx_token_embedding_forward(int32_t dtype, const int64_t* index, int64_t n, const void* table, int64_t V,
+                                 int64_t D, float scale, void* out, aimx_stream_t stream);
+size_t aimx_token_embedding_backward_workspace_bytes(int32_t dtype, int64_t n, int64_t V, int64_t D);
+int aimx_token_embedding_backward(int32_t dtype, const int64_t* index, int64_t n, const void* dy, int64_t ldd,
+                                  int64_t V, int64_t D, float scale, int64_t padding_idx, void* dtable,
+                                  void* workspace, size_t workspace_bytes, aimx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Gradient all-reduce over RCCL (xGMI inside an MI355X node) — the DDP reducer's collective
  * (reference runner.py:703-707 wraps the model in DistributedDataParallel over "nccl" = RCCL).
  * RCCL is resolved at run time (aimx_comm_load: dlopen of the RCCL the process already uses, e.g.
