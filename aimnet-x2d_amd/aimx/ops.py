@@ -1255,7 +1255,7 @@ def _dense_forward(x, ws, bs, res, act, prec, keep_pre):
         d.res = ptr(r2)
     pre = None
     if keep_pre:
-        pre = torch.empty(d.M, len(ws) * n, dtype=_F32, device=dev)
+        pre = torch.empty(d.M, len(ws), -(-n // 8) * 8, dtype=_F32, device=dev)
         d.pre = ptr(pre)
     with _on(dev):
         d.workspace_bytes = lib.aimx_dense_workspace_bytes(ctypes.byref(d))
@@ -1267,7 +1267,8 @@ def _dense_forward(x, ws, bs, res, act, prec, keep_pre):
 
 class _DenseFn(torch.autograd.Function):
     """halves = 1: dense(x, w, b, residual); halves = 2: gated_linear(x, w_gate, w_up, b_gate, b_up). Kept for
-    the backward: x (or its 8-bit form) and, unless checkpoint8, the fp32 values before the activation."""
+    the backward: x (or its 8-bit form) and, for fp32 products without checkpoint8, the values before the
+    activation."""
 
     @staticmethod
     def forward(ctx, x, w0, w1, b0, b1, res, act, checkpoint8):
@@ -1275,7 +1276,9 @@ class _DenseFn(torch.autograd.Function):
         bs = [b.contiguous() if b is not None else None for b in ((b0, b1) if w1 is not None else (b0,))]
         ctx.prec = amp_precision() if x.dtype == _F32 else PREC_FP32
         need = ctx.needs_input_grad
-        y, pre, x2 = _dense_forward(x, ws, bs, res, act, ctx.prec, act >= 0 and not checkpoint8 and any(need[:5]))
+        # bf16 products compute the values before the activation again; fp32 ones are worth keeping
+        keep = x.dtype == _F32 and ctx.prec == PREC_FP32 and act >= 0 and not checkpoint8 and any(need[:5])
+        y, pre, x2 = _dense_forward(x, ws, bs, res, act, ctx.prec, keep)
         ctx.act, ctx.shape, ctx.halves = act, x.shape, len(ws)
         kept, exps = x2, None
         if checkpoint8:
@@ -1365,8 +1368,8 @@ def dense(x, w, b=None, act=None, residual=None, checkpoint8=False):
     """y = act(x w^T + b) + residual in one kernel: x [..., n_in], w [n_out, n_in], b [n_out] or None, act None
     or an activation name, residual [..., n_out] or None; all fp32 or all bf16. fp32 at fp32 accuracy
     (bf16 operands inside torch.autocast, as linear()). Differentiable in every tensor.
-    checkpoint8=True: the backward keeps x in 8 bits (pack8: 33/32 bytes a value) instead of x and the
-    values before the activation, and computes the gradients for the x that those bits stand for."""
+    checkpoint8=True: what is kept for the backward is x in 8 bits (pack8: 33/32 bytes a value) instead of x
+    (fp32: and the values before the activation); the gradients are those at the x that the bits stand for."""
     kind = _dense_checks("dense", x, [w], [b], act, residual)
     return _dense_apply("dense", x, [w], [b], residual, kind, checkpoint8)
 

@@ -7,9 +7,10 @@
 //   dP = dy act'(p)    |    dG = dy u act'(g), dU = dy act(g)
 //   dx = dP W          |    dx = dG Wg + dU Wu, one product over both halves' columns
 //   dW = dP^T x, db = column sums of dP (fp32, before dP is rounded)
-// Every product is D[m][n] = sum_k A[m][k] B[n][k] (dense_core.h); the operands whose rows run along the
-// wrong axis are transposed while they are staged: the kernels below also pad, split fp32 into planes and
-// unpack 8-bit values, in the one pass over them that this needs.
+// Every product is D[m][n] = sum_k A[m][k] B[n][k] (dense_core.h), dx and dW with operands read across their rows.
+// bf16 tensors: the backward does not read kept pre-activations, it runs the forward product again with an epilogue
+// that leaves dP / [dG | dU]: at 20480 x 512 -> 2 x 2048 that is 86 GF, where fp32 values before the activation
+// would be 335 MB written and read again. fp32 tensors keep them: their product costs six times as much.
 //
 // Roundings to fewer bits: y, dx, dW and db once, to the tensors' type. bf16 tensors: dP / dG / dU are
 // rounded to bf16 for the matrix instructions (their sums for db are not); with the result's own rounding
@@ -34,6 +35,7 @@ struct Segment {
   uint16_t* dst;
   int64_t ldd, plane;
   int64_t first;  // first work item of this segment
+  int32_t vec;    // 16-byte loads (kQ8: 8-byte ones, always)
 };
 struct Segments {
   Segment s[3];
@@ -41,17 +43,30 @@ struct Segments {
   int64_t items;
 };
 
-template <int SRC>
-__device__ __forceinline__ float source(const Segment& s, int64_t r, int64_t c) {
-  if constexpr (SRC == kF32) return ((const float*)s.src)[r * s.ld + c];
-  if constexpr (SRC == kBf16) return from_bf16(((const uint16_t*)s.src)[r * s.ld + c]);
-  const int e = s.exp[r * ((s.C + 31) / 32) + c / 32];
-  return e == 127 ? __uint_as_float(0x7fc00000u) : ldexpf((float)((const int8_t*)s.src)[r * s.ld + c], e);
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef int8_t i8x8 __attribute__((ext_vector_type(8)));
+
+// 8 values from p, `left` of which exist (the others: zero)
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int64_t left, float (&v)[8]) {
+  if (vec && left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+      const u16x8 a = *reinterpret_cast<const u16x8*>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from_bf16(a[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? load1(p + i) : 0.f;
+  }
 }
 
 template <int PL>
 __device__ __forceinline__ void store_planes8(uint16_t* dst, int64_t plane, const float (&v)[8]) {
-  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
   u16x8 o[PL];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -68,125 +83,86 @@ __device__ __forceinline__ void store_planes8(uint16_t* dst, int64_t plane, cons
   for (int q = 0; q < PL; ++q) *reinterpret_cast<u16x8*>(dst + q * plane) = o[q];
 }
 
-__device__ __forceinline__ const Segment& segment_of(const Segments& a, int64_t item) {
-  int k = 0;
-  while (k + 1 < a.n && a.s[k + 1].first <= item) ++k;
-  return a.s[k];
-}
-
-// Rows as they are: planes [PL][R][ldd], zeros behind column C. An item is 8 columns of a row.
+// Planes [PL][R][ldd], zeros behind column C. An item is 8 columns of a row.
 template <int SRC, int PL>
 __global__ __launch_bounds__(256) void k_stage(const Segments a) {
   for (int64_t item = blockIdx.x * (int64_t)256 + threadIdx.x; item < a.items; item += (int64_t)gridDim.x * 256) {
-    const Segment& s = segment_of(a, item);
+    int k = 0;
+    while (k + 1 < a.n && a.s[k + 1].first <= item) ++k;
+    const Segment& s = a.s[k];
     const int64_t w = s.ldd / 8, i = item - s.first, r = i / w, c = (i - r * w) * 8;
     float v[8];
+    if constexpr (SRC == kQ8) {
+      const int e = c < s.C ? s.exp[r * ((s.C + 31) / 32) + c / 32] : 0;
+      i8x8 q = {};
+      if (c < s.C) q = *reinterpret_cast<const i8x8*>((const int8_t*)s.src + r * s.ld + c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < s.C ? source<SRC>(s, r, c + e) : 0.f;
+      for (int j = 0; j < 8; ++j)
+        v[j] = c + j < s.C ? (e == 127 ? __uint_as_float(0x7fc00000u) : ldexpf((float)q[j], e)) : 0.f;
+    } else if constexpr (SRC == kF32) {
+      load8((const float*)s.src + r * s.ld + c, s.vec, s.C - c, v);
+    } else {
+      load8((const uint16_t*)s.src + r * s.ld + c, s.vec, s.C - c, v);
+    }
     store_planes8<PL>(s.dst + r * s.ldd + c, s.plane, v);
   }
 }
 
-// Transposed: dst[c][r], planes of [C][ldd], zeros for R <= r < up64(R). An item is a 64 x 64 tile.
-template <int SRC, int PL>
-__global__ __launch_bounds__(256) void k_stage_t(const Segments a) {
-  __shared__ float tile[64][65];
-  const Segment& s = segment_of(a, blockIdx.x);
-  const int64_t tc = (s.C + 63) / 64, i = blockIdx.x - s.first, r0 = i / tc * 64, c0 = (i - i / tc * tc) * 64;
-  {
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int64_t rr = r0 + r + 4 * j, cc = c0 + c;
-      tile[r + 4 * j][c] = rr < s.R && cc < s.C ? source<SRC>(s, rr, cc) : 0.f;
-    }
-  }
-  __syncthreads();
-  const int r8 = (threadIdx.x & 7) * 8;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int c = (threadIdx.x >> 3) + 32 * j;
-    if (c0 + c >= s.C) continue;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[r8 + e][c];
-    store_planes8<PL>(s.dst + (c0 + c) * s.ldd + r0 + r8, s.plane, v);
-  }
-}
-
-// The gradient before the activation: rows [PL][M][halves * Np] (the first operand of dx), transposed
-// [PL][halves * N][Mp] (the first operand of dW) and each 64-row tile's column sums, whichever is asked for.
+// The gradient before the activation from kept values, or dy itself: planes [PL][M][halves * Np] with zeros behind
+// column N (nullptr: not wanted), and the column sums of each 128 rows (nullable).
 struct Dpre {
   const void* dy;
-  int64_t ldd, M, N, Np, Mp;
-  const float* pre;  // [M][halves * N]; nullptr: no activation
+  int64_t ldd, M, N, Np, N8;
+  const float* pre;  // [M][halves][N8]; nullptr: no activation
   uint16_t* rows;
-  uint16_t* cols;
-  int64_t rows_plane, cols_plane;
-  float* sums;  // [cdiv(M, 64)][halves * N]
-  int32_t act;
+  int64_t plane;
+  float* sums;  // [cdiv(M, 128)][halves * N]
+  int32_t act, vec;
 };
+constexpr int kDpreRows = 128;
 template <typename T, int PL, int HALVES>
 __global__ __launch_bounds__(256) void k_dpre(const Dpre a) {
-  __shared__ float tile[HALVES][64][65];
-  __shared__ float part[HALVES][4][64];
-  const int64_t tn = a.Np / 64, tm = blockIdx.x / tn, m0 = tm * 64, n0 = (blockIdx.x - tm * tn) * 64;
-  {
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-    const int64_t n = n0 + c;
+  __shared__ float part[HALVES][32][65];
+  const int64_t tn = a.Np / 64, tm = blockIdx.x / tn;
+  const int c8 = (threadIdx.x & 7) * 8, r = threadIdx.x >> 3;
+  const int64_t n = (blockIdx.x - tm * tn) * 64 + c8;
+  float total[HALVES][8] = {};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int64_t m = m0 + r + 4 * j;
-      const bool ok = m < a.M && n < a.N;
-      float d = ok ? load1((const T*)a.dy + m * a.ldd + n) : 0.f;
-      if constexpr (HALVES == 2) {
-        float dg = 0.f, du = 0.f;
-        if (ok) {
-          const float g = a.pre[m * 2 * a.N + n], u = a.pre[m * 2 * a.N + a.N + n];
-          dg = d * u * act_grad(a.act, g);
-          du = d * act_fwd(a.act, g);
-        }
-        tile[0][r + 4 * j][c] = dg;
-        tile[1][r + 4 * j][c] = du;
-      } else {
-        if (ok && a.pre) d *= act_grad(a.act, a.pre[m * a.N + n]);
-        tile[0][r + 4 * j][c] = d;
-      }
+  for (int j = 0; j < kDpreRows / 32; ++j) {
+    const int64_t m = tm * kDpreRows + j * 32 + r;
+    if (m >= a.M) continue;
+    float d[8], g[8], u[8], o[8];
+    load8((const T*)a.dy + m * a.ldd + n, a.vec, a.N - n, d);
+    if (a.pre && n < a.N8) {
+      load8(a.pre + m * HALVES * a.N8 + n, true, 8, g);
+      if constexpr (HALVES == 2) load8(a.pre + m * HALVES * a.N8 + a.N8 + n, true, 8, u);
     }
-  }
-  __syncthreads();
-  const int e8 = (threadIdx.x & 7) * 8;
 #pragma unroll
-  for (int h = 0; h < HALVES; ++h) {
+    for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int t = (threadIdx.x >> 3) + 32 * j;
-      float v[8];
-      if (a.rows && m0 + t < a.M) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[h][t][e8 + e];
-        store_planes8<PL>(a.rows + (m0 + t) * HALVES * a.Np + h * a.Np + n0 + e8, a.rows_plane, v);
+      for (int e = 0; e < 8; ++e) {
+        o[e] = d[e];
+        if (n + e >= a.N) continue;  // behind N: d is zero, pre undefined
+        if constexpr (HALVES == 2) o[e] = h == 0 ? d[e] * u[e] * act_grad(a.act, g[e]) : d[e] * act_fwd(a.act, g[e]);
+        else if (a.pre) o[e] = d[e] * act_grad(a.act, g[e]);
+        total[h][e] += o[e];
       }
-      if (a.cols && n0 + t < a.N) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[h][e8 + e][t];
-        store_planes8<PL>(a.cols + (h * a.N + n0 + t) * a.Mp + m0 + e8, a.cols_plane, v);
-      }
-    }
-    if (a.sums) {
-      const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s += tile[h][w * 16 + i][c];
-      part[h][w][c] = s;
+      if (a.rows) store_planes8<PL>(a.rows + m * HALVES * a.Np + h * a.Np + n, a.plane, o);
     }
   }
   if (!a.sums) return;
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[h][r][c8 + e] = total[h][e];
   __syncthreads();
   if (threadIdx.x < 64 * HALVES) {
     const int h = threadIdx.x >> 6, c = threadIdx.x & 63;
-    if (n0 + c < a.N)
-      a.sums[tm * HALVES * a.N + h * a.N + n0 + c] = (part[h][0][c] + part[h][1][c]) + (part[h][2][c] + part[h][3][c]);
+    const int64_t col = (blockIdx.x - tm * tn) * 64 + c;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += part[h][i][c];
+    if (col < a.N) a.sums[tm * HALVES * a.N + h * a.N + col] = s;
   }
 }
 
@@ -222,15 +198,14 @@ __global__ __launch_bounds__(256) void k_reduce_slabs(const Problem p) {
     floatx4 v = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < p.splits; ++s) v += load4(p.slab + ((int64_t)s * p.M + m) * p.N + n, v4, left);
     if (p.bias) v += load4((const T*)p.bias + n, v4, left);
-    if (p.pre) store4(p.pre + m * p.N + n, v, v4, left);
-    if (!p.y) continue;
+    if (p.pre) *reinterpret_cast<floatx4*>(p.pre + m * p.n8 + n) = v;
     if (p.act >= 0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = act_fwd(p.act, v[e]);
     }
     if (p.res) v += load4((const T*)p.res + m * p.ldr + n, v4, left);
-    T* y = m < p.y_rows ? (T*)p.y + m * p.ldy : (T*)p.y2 + (m - p.y_rows) * p.ldy;
-    store4(y + n, v, v4, left);
+    const int64_t r = m < p.y_rows ? m : m - p.y_rows;
+    if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, v, v4, left);
   }
 }
 
@@ -258,37 +233,33 @@ struct Ctx {
 };
 
 template <int SRC, int PL>
-void stage_go(Ctx& c, Segments& a, bool transpose) {
-  if (a.items == 0) return;
-  if (transpose)
-    hipLaunchKernelGGL((k_stage_t<SRC, PL>), dim3((unsigned)a.items), dim3(256), 0, c.st, a);
-  else
-    hipLaunchKernelGGL((k_stage<SRC, PL>), dim3((unsigned)std::min<int64_t>(cdiv(a.items, 256), 16384)), dim3(256), 0,
-                       c.st, a);
+void stage_go(Ctx& c, const Segments& a) {
+  hipLaunchKernelGGL((k_stage<SRC, PL>), dim3((unsigned)std::min<int64_t>(cdiv(a.items, 256), 16384)), dim3(256), 0,
+                     c.st, a);
   c.rc = (int)hipGetLastError();
 }
 
 // Launches a list of segments of one kind of source.
-void stage(Ctx& c, Segments& a, int src, int planes, bool transpose) {
+void stage(Ctx& c, Segments& a, int src, int planes) {
   if (c.dry || c.rc || a.n == 0) return;
   a.items = 0;
   for (int i = 0; i < a.n; ++i) {
     a.s[i].first = a.items;
-    a.items += transpose ? cdiv(a.s[i].R, 64) * cdiv(a.s[i].C, 64) : a.s[i].R * (a.s[i].ldd / 8);
+    a.items += a.s[i].R * (a.s[i].ldd / 8);
+    a.s[i].vec = aligned16(a.s[i].src) && a.s[i].ld % (src == kF32 ? 4 : 8) == 0;
   }
-  if (transpose && a.items > INT32_MAX) {
-    c.rc = AIMX_EARG;
-    return;
-  }
-  if (src == kF32) return planes == 3 ? stage_go<kF32, 3>(c, a, transpose) : stage_go<kF32, 1>(c, a, transpose);
-  if (src == kBf16) return stage_go<kBf16, 1>(c, a, transpose);
-  return stage_go<kQ8, 1>(c, a, transpose);
+  if (a.items == 0) return;
+  if (src == kF32) return planes == 3 ? stage_go<kF32, 3>(c, a) : stage_go<kF32, 1>(c, a);
+  if (src == kBf16) return stage_go<kBf16, 1>(c, a);
+  return stage_go<kQ8, 1>(c, a);
 }
 
-void product(Ctx& c, Carve& ws, Problem p, int pa, int pb, int halves, bool fp32, bool may_split) {
+// One product and, where its k is split, the sum of its parts.
+void product(Ctx& c, Carve& ws, Problem p, int pa, int pb, int epi, int across, bool fp32) {
   if (p.M == 0) return;
   const bool one = pa == 1 && pb == 1;
-  const Plan t = one ? plan_one(p.M, p.N * halves, p.K, may_split) : plan_split(p.M, p.N * halves, p.K, may_split);
+  const int halves = epi == kGated || epi == kGatedGrad ? 2 : 1;
+  const Plan t = one ? plan_one(p.M, p.N * halves, p.K, epi == kPlain) : plan_split(p.M, p.N * halves, p.K, epi == kPlain);
   p.splits = t.splits;
   if (t.splits > 1) p.slab = ws.take<float>((int64_t)t.splits * p.M * p.N);
   if (c.dry || c.rc) return;
@@ -296,9 +267,12 @@ void product(Ctx& c, Carve& ws, Problem p, int pa, int pb, int halves, bool fp32
   const size_t b = fp32 ? 4 : 2;
   auto four = [&](const void* q, int64_t ld) { return !q || (((uintptr_t)q % (4 * b)) == 0 && ld % 4 == 0); };
   p.vec = p.N % 4 == 0 && four(p.y, p.ldy) && four(p.y2, p.ldy) && four(p.res, p.ldr) && four(p.bias, 0) &&
-          four(p.bias2, 0) && aligned16(p.pre);
-  if (p.y_rows == 0) p.y_rows = p.M;
-  c.rc = one ? launch_one(p, t.tile, halves, fp32, c.st) : launch_split(p, t.tile, pa, pb, halves, c.st);
+          four(p.bias2, 0);
+  p.n8 = (p.N + 7) / 8 * 8;
+  p.np = up64(p.N);
+  if (p.k_half == 0) p.k_half = p.K;
+  if (p.y_rows == 0) p.y_rows = p.y_valid = p.M;
+  c.rc = one ? launch_one(p, t.tile, epi, across, fp32, c.st) : launch_split(p, t.tile, pa, pb, epi, across, c.st);
   if (c.rc || t.splits == 1) return;
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(p.M * cdiv(p.N, 4), 256), 16384));
   if (fp32) hipLaunchKernelGGL(k_reduce_slabs<float>, grid, dim3(256), 0, c.st, p);
@@ -329,68 +303,68 @@ Kind kind_of(const AimxDense* d) {
   return {f, f && d->precision == AIMX_PREC_FP32 ? 3 : 1, f ? kF32 : kBf16, f ? (size_t)4 : (size_t)2};
 }
 
-// a bf16 matrix the products can read where it is
-bool in_place(const Kind& k, const void* p, int64_t ld, int64_t cols) {
-  return !k.fp32 && aligned16(p) && ld % 8 == 0 && cols % 64 == 0;
+// a bf16 matrix the products can read where it is, along its rows (k contiguous) or across them
+bool in_place(const Kind& k, const void* p, int64_t ld, int64_t cols, bool along) {
+  return !k.fp32 && aligned16(p) && ld % 8 == 0 && cols % (along ? 64 : 8) == 0;
 }
 
-Segment& add(Segments& a, const void* src, int64_t ld, int64_t R, int64_t C, uint16_t* dst, int64_t ldd, int64_t plane) {
-  Segment& s = a.s[a.n++];
-  s = Segment{src, nullptr, ld, R, C, dst, ldd, plane, 0};
-  return s;
+void add(Segments& a, const void* src, const int8_t* exp, int64_t ld, int64_t R, int64_t C, uint16_t* dst, int64_t ldd) {
+  a.s[a.n++] = Segment{src, exp, ld, R, C, dst, ldd, R * ldd, 0, 0};
 }
 
-// x W^T with the forward's epilogue. From the 8-bit form of x where d->x is null. w_only: y is not
-// written, only pre.
-void forward(Ctx& c, Carve& ws, const AimxDense* d, float* pre, bool pre_only) {
-  const Kind k = kind_of(d);
+// x (or its 8-bit form) as an operand; `along` if some product reads it along its rows
+Operand operand_x(const AimxDense* d, const Kind& k, Carve& ws, bool along, Segments& same, Segments& eight) {
+  if (d->x && in_place(k, d->x, d->ldx, d->K, along)) return {(const uint16_t*)d->x, nullptr, d->ldx, 0, d->M, d->K};
   const int64_t Kp = up64(d->K);
+  uint16_t* t = ws.take<uint16_t>(d->M * Kp * (d->x ? k.planes : 1));
+  if (d->x) add(same, d->x, nullptr, d->ldx, d->M, d->K, t, Kp);
+  else add(eight, d->q, d->qexp, (d->K + 31) / 32 * 32, d->M, d->K, t, Kp);
+  return {t, nullptr, Kp, d->M * Kp, d->M, Kp};
+}
+
+Operand operand_w(const AimxDense* d, const Kind& k, Carve& ws, bool along, Segments& same) {
+  if (in_place(k, d->w[0], d->ldw, d->K, along) && (d->halves == 1 || aligned16(d->w[1])))
+    return {(const uint16_t*)d->w[0], (const uint16_t*)d->w[1], d->ldw, 0, d->N, d->K};
+  const int64_t Kp = up64(d->K);
+  uint16_t* t[2] = {nullptr, nullptr};
+  for (int h = 0; h < d->halves; ++h) {
+    t[h] = ws.take<uint16_t>(d->N * Kp * k.planes);
+    add(same, d->w[h], nullptr, d->ldw, d->N, d->K, t[h], Kp);
+  }
+  return {t[0], t[1], Kp, d->N * Kp, d->N, Kp};
+}
+
+// the forward product's problem
+Problem forward_problem(const AimxDense* d, const Operand& x, const Operand& w) {
   Problem p{};
+  p.a = x;
+  p.b = w;
   p.M = d->M;
   p.N = d->N;
-  p.K = Kp;
+  p.K = up64(d->K);
   p.act = d->act;
-  p.pre = pre;
-  if (!pre_only) {
-    p.y = d->y;
-    p.ldy = d->ldy;
-    p.res = d->res;
-    p.ldr = d->ldr;
-  }
   p.bias = d->b[0];
   p.bias2 = d->b[1];
-  Segments same{}, eight{};
-  int pa = k.planes;
-  p.a = Operand{(const uint16_t*)d->x, nullptr, d->ldx, 0, d->M};
-  if (!d->x) {
-    pa = 1;
-    uint16_t* t = ws.take<uint16_t>(d->M * Kp);
-    p.a = Operand{t, nullptr, Kp, 0, d->M};
-    add(eight, d->q, (d->K + 31) / 32 * 32, d->M, d->K, t, Kp, 0).exp = d->qexp;
-  } else if (!in_place(k, d->x, d->ldx, d->K)) {
-    const int64_t plane = d->M * Kp;
-    uint16_t* t = ws.take<uint16_t>(plane * k.planes);
-    p.a = Operand{t, nullptr, Kp, plane, d->M};
-    add(same, d->x, d->ldx, d->M, d->K, t, Kp, plane);
-  }
-  p.b = Operand{(const uint16_t*)d->w[0], (const uint16_t*)d->w[1], d->ldw, 0, d->N};
-  if (!in_place(k, d->w[0], d->ldw, d->K) || (d->halves == 2 && !aligned16(d->w[1]))) {
-    const int64_t plane = d->N * Kp;
-    uint16_t* t[2] = {nullptr, nullptr};
-    for (int h = 0; h < d->halves; ++h) {
-      t[h] = ws.take<uint16_t>(plane * k.planes);
-      add(same, d->w[h], d->ldw, d->N, d->K, t[h], Kp, plane);
-    }
-    p.b = Operand{t[0], t[1], Kp, plane, d->N};
-  }
-  stage(c, same, k.src, k.planes, false);
-  stage(c, eight, kQ8, 1, false);
-  product(c, ws, p, pa, k.planes, d->halves, k.fp32, d->halves == 1);
+  return p;
+}
+
+void forward(Ctx& c, Carve& ws, const AimxDense* d) {
+  const Kind k = kind_of(d);
+  Segments same{}, none{};
+  const Operand x = operand_x(d, k, ws, true, same, none), w = operand_w(d, k, ws, true, same);
+  stage(c, same, k.src, k.planes);
+  Problem p = forward_problem(d, x, w);
+  p.y = d->y;
+  p.ldy = d->ldy;
+  p.res = d->res;
+  p.ldr = d->ldr;
+  p.pre = d->pre;
+  product(c, ws, p, k.planes, k.planes, d->halves == 2 ? kGated : kPlain, kNone, k.fp32);
 }
 
 template <typename T, int PL>
 void dpre_go(Ctx& c, const Dpre& a, int halves) {
-  const dim3 grid((unsigned)(a.Np / 64 * cdiv(a.M, 64)));
+  const dim3 grid((unsigned)(a.Np / 64 * cdiv(a.M, kDpreRows)));
   if (halves == 2) hipLaunchKernelGGL((k_dpre<T, PL, 2>), grid, dim3(256), 0, c.st, a);
   else hipLaunchKernelGGL((k_dpre<T, PL, 1>), grid, dim3(256), 0, c.st, a);
   c.rc = (int)hipGetLastError();
@@ -398,95 +372,97 @@ void dpre_go(Ctx& c, const Dpre& a, int halves) {
 
 void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
   const Kind k = kind_of(d);
-  const int64_t M = d->M, N = d->N, K = d->K, H = d->halves, Np = up64(N), Mp = up64(M);
+  const int64_t M = d->M, N = d->N, K = d->K, H = d->halves, Np = up64(N);
   const bool has_dw = g->dw[0] != nullptr, has_db = g->db[0] != nullptr, has_dx = g->dx != nullptr;
-  const float* pre = d->pre;
-  if (d->act >= 0 && !pre) {
-    float* t = ws.take<float>(M * H * N);
-    forward(c, ws, d, t, true);
-    pre = t;
-  }
-  Dpre a{};
-  a.dy = g->dy;
-  a.ldd = g->ldd;
-  a.M = M;
-  a.N = N;
-  a.Np = Np;
-  a.Mp = Mp;
-  a.act = d->act;
-  a.pre = d->act >= 0 ? pre : nullptr;
-  Operand rows{};
-  if (has_dx) {
-    if (d->act < 0 && in_place(k, g->dy, g->ldd, N)) {
-      rows = Operand{(const uint16_t*)g->dy, nullptr, g->ldd, 0, M};
-    } else {
-      a.rows_plane = M * H * Np;
-      a.rows = ws.take<uint16_t>(a.rows_plane * k.planes);
-      rows = Operand{a.rows, nullptr, H * Np, a.rows_plane, M};
+  const bool again = d->act >= 0 && !d->pre;  // the values before the activation are computed again
+  const int px = d->x ? k.planes : 1;
+  Segments same{}, eight{};
+  Operand x{}, w{}, rows{};
+  if (has_dw || again) x = operand_x(d, k, ws, again, same, eight);
+  if (has_dx || again) w = operand_w(d, k, ws, again, same);
+  stage(c, same, k.src, k.planes);
+  stage(c, eight, kQ8, 1);
+
+  // dP / [dG | dU] as an operand and the parts of its column sums
+  const int64_t plane = M * H * Np;
+  const float* sums = nullptr;
+  int64_t parts = 0;
+  if (again) {
+    uint16_t* t = ws.take<uint16_t>(plane * k.planes);
+    rows = {t, nullptr, H * Np, plane, M, H * Np};
+    Problem p = forward_problem(d, x, w);
+    p.res = g->dy;
+    p.ldr = g->ldd;
+    p.rows = t;
+    p.rows_plane = plane;
+    const Plan at = (px == 1 && k.planes == 1) ? plan_one(M, N * H, p.K, false) : plan_split(M, N * H, p.K, false);
+    parts = cdiv(M, at.tile_m) * at.waves_m;
+    if (has_db) sums = p.sums = ws.take<float>(parts * H * N);
+    product(c, ws, p, px, k.planes, H == 2 ? kGatedGrad : kDenseGrad, kNone, k.fp32);
+  } else {
+    Dpre a{};
+    a.dy = g->dy;
+    a.ldd = g->ldd;
+    a.M = M;
+    a.N = N;
+    a.Np = Np;
+    a.N8 = (N + 7) / 8 * 8;
+    a.pre = d->act >= 0 ? d->pre : nullptr;
+    a.act = d->act;
+    a.vec = aligned16(g->dy) && g->ldd % (k.fp32 ? 4 : 8) == 0;
+    if (d->act < 0 && in_place(k, g->dy, g->ldd, N, has_dx)) {
+      rows = {(const uint16_t*)g->dy, nullptr, g->ldd, 0, M, N};
+    } else if (has_dx || has_dw) {
+      a.rows = ws.take<uint16_t>(plane * k.planes);
+      a.plane = plane;
+      rows = {a.rows, nullptr, H * Np, plane, M, H * Np};
     }
-  }
-  if (has_dw) {
-    a.cols_plane = H * N * Mp;
-    a.cols = ws.take<uint16_t>(a.cols_plane * k.planes);
-  }
-  if (has_db) a.sums = ws.take<float>(cdiv(M, 64) * H * N);
-  if (!c.dry && !c.rc && M > 0 && (a.rows || a.cols || a.sums)) {
-    if (Np / 64 * cdiv(M, 64) > INT32_MAX) c.rc = AIMX_EARG;
-    else if (!k.fp32) dpre_go<uint16_t, 1>(c, a, (int)H);
-    else if (k.planes == 3) dpre_go<float, 3>(c, a, (int)H);
-    else dpre_go<float, 1>(c, a, (int)H);
+    parts = cdiv(M, kDpreRows);
+    if (has_db) sums = a.sums = ws.take<float>(parts * H * N);
+    if (!c.dry && !c.rc && M > 0 && (a.rows || a.sums)) {
+      if (Np / 64 * parts > INT32_MAX) c.rc = AIMX_EARG;
+      else if (!k.fp32) dpre_go<uint16_t, 1>(c, a, (int)H);
+      else if (k.planes == 3) dpre_go<float, 3>(c, a, (int)H);
+      else dpre_go<float, 1>(c, a, (int)H);
+    }
   }
   if (has_db && !c.dry && !c.rc) {
     const dim3 grid((unsigned)cdiv(H * N, 64));
     if (k.fp32)
-      hipLaunchKernelGGL(k_column_sums<float>, grid, dim3(1024), 0, c.st, a.sums, cdiv(M, 64), N, (int)H,
-                         (float*)g->db[0], (float*)g->db[1]);
+      hipLaunchKernelGGL(k_column_sums<float>, grid, dim3(1024), 0, c.st, sums, parts, N, (int)H, (float*)g->db[0],
+                         (float*)g->db[1]);
     else
-      hipLaunchKernelGGL(k_column_sums<uint16_t>, grid, dim3(1024), 0, c.st, a.sums, cdiv(M, 64), N, (int)H,
+      hipLaunchKernelGGL(k_column_sums<uint16_t>, grid, dim3(1024), 0, c.st, sums, parts, N, (int)H,
                          (uint16_t*)g->db[0], (uint16_t*)g->db[1]);
     c.rc = (int)hipGetLastError();
   }
-  // the transposed x (or its 8-bit form) and weights
-  Segments same{}, eight{};
-  uint16_t *xt = nullptr, *wt = nullptr;
-  const int64_t xplane = K * Mp, wplane = K * H * Np;
-  const int px = d->x ? k.planes : 1;
-  if (has_dw) {
-    xt = ws.take<uint16_t>(xplane * px);
-    if (d->x) add(same, d->x, d->ldx, M, K, xt, Mp, xplane);
-    else add(eight, d->q, (K + 31) / 32 * 32, M, K, xt, Mp, 0).exp = d->qexp;
-  }
-  if (has_dx) {
-    wt = ws.take<uint16_t>(wplane * k.planes);
-    for (int h = 0; h < H; ++h) add(same, d->w[h], d->ldw, N, K, wt ? wt + h * Np : nullptr, H * Np, wplane);
-  }
-  stage(c, same, k.src, k.planes, true);
-  stage(c, eight, kQ8, 1, true);
   if (has_dx) {
     Problem p{};
     p.a = rows;
-    p.b = Operand{wt, nullptr, H * Np, wplane, K};
+    p.b = w;
     p.M = M;
     p.N = K;
     p.K = H * Np;
+    p.k_half = Np;
     p.y = g->dx;
     p.ldy = g->lddx;
     p.act = AIMX_ACT_NONE;
-    product(c, ws, p, k.planes, k.planes, 1, k.fp32, true);
+    product(c, ws, p, k.planes, k.planes, kPlain, kB, k.fp32);
   }
   if (has_dw) {
     Problem p{};
-    p.a = Operand{a.cols, nullptr, Mp, a.cols_plane, H * N};
-    p.b = Operand{xt, nullptr, Mp, xplane, K};
-    p.M = H * N;
+    p.a = rows;
+    p.b = x;
+    p.M = H == 2 ? H * Np : N;
     p.N = K;
-    p.K = Mp;
+    p.K = up64(M);
     p.y = g->dw[0];
     p.y2 = g->dw[1];
     p.ldy = K;
-    p.y_rows = N;
+    p.y_rows = H == 2 ? Np : N;
+    p.y_valid = N;
     p.act = AIMX_ACT_NONE;
-    product(c, ws, p, k.planes, px, 1, k.fp32, true);
+    product(c, ws, p, k.planes, px, kPlain, kBoth, k.fp32);
   }
 }
 
@@ -497,7 +473,10 @@ bool valid_grad(const AimxDense* d, const AimxDenseGrad* g) {
     return false;
   if ((d->M > 0 && !g->dy) || g->ldd < d->N || (g->dx && g->lddx < d->K) || g->ldd > (int64_t)1 << 21) return false;
   if (d->M > (int64_t)1 << 22) return false;  // the transposed operands' rows run along M
-  return d->M == 0 || d->x || (d->q && d->qexp);
+  if (d->pre && ((uintptr_t)d->pre & 15)) return false;
+  if (!d->x) return d->M == 0 || (d->q && d->qexp && ((uintptr_t)d->q & 7) == 0);
+  // fp32 products keep the values before the activation where they keep x
+  return d->act < 0 || d->pre || kind_of(d).planes == 1;
 }
 
 }  // namespace
@@ -510,18 +489,18 @@ extern "C" size_t aimx_dense_workspace_bytes(const AimxDense* d) {
   if (!dense::valid(d)) return 0;
   dense::Ctx c{nullptr, true};
   dense::Carve ws{nullptr};
-  dense::forward(c, ws, d, d->pre, false);
+  dense::forward(c, ws, d);
   return ws.used;
 }
 
 extern "C" int aimx_dense_forward(const AimxDense* d, aimx_stream_t stream) {
-  if (!dense::valid(d) || (d->M > 0 && (!d->x || !d->y)) || d->ldy < d->N) return AIMX_EARG;
+  if (!dense::valid(d) || (d->M > 0 && (!d->x || !d->y)) || d->ldy < d->N || !dense::aligned16(d->pre)) return AIMX_EARG;
   if (d->M == 0) return AIMX_OK;
   if (d->workspace_bytes < aimx_dense_workspace_bytes(d) || (d->workspace_bytes && !d->workspace)) return AIMX_EARG;
   if (!dense::aligned16(d->workspace)) return AIMX_EARG;
   dense::Ctx c{(hipStream_t)stream, false};
   dense::Carve ws{(char*)d->workspace};
-  dense::forward(c, ws, d, d->pre, false);
+  dense::forward(c, ws, d);
   return c.rc;
 }
 

@@ -9,9 +9,13 @@
 // fp32. Six bf16 instructions replace sixteen times slower fp32 ones. Against a one-plane operand three
 // plane products are the whole product.
 //
-// Layout rules (the host stages operands that break them): rows 16-byte aligned, k contiguous, ld and the
-// k extent multiples of 64 elements with zeros behind the matrix's own columns. Rows are guarded by the
-// buffer descriptors: a row past the end reads zeros.
+// An operand is read along its rows (k contiguous) or across them: a matrix whose rows run along k (the
+// weight in dx, both operands in dW) goes into LDS as it is and is transposed by the fragment reads
+// (ds_read_b64_tr_b16), so no product needs a transposed copy.
+//
+// Layout rules (the host stages operands that break them): rows 16-byte aligned. Along the rows: the k extent a
+// multiple of 64 elements, zeros behind the matrix's own columns. Across: columns a multiple of 8. Rows and k
+// past the end read zeros through the buffer descriptors, which end with the matrix.
 #pragma once
 
 #include <algorithm>
@@ -49,30 +53,39 @@ __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
   p[2] = to_bf16(r1 - from_bf16(p[1]));
 }
 
-// One operand of a product. `half` rows come from p, the rows behind them from p2 (the gated forward's two
-// weights); plane q is at + q * plane elements.
+// One operand of a product: `rows` rows of `cols` elements, planes `plane` elements apart. p2: the second weight (the
+// gated forward's second half of columns; across the rows, the second half of k).
 struct Operand {
   const uint16_t* p;
   const uint16_t* p2;
-  int64_t ld, plane, rows;
+  int64_t ld, plane, rows, cols;
 };
 
 struct Problem {
   Operand a, b;
   int64_t M, N, K;       // N: columns of the result (of one half where the epilogue is gated); K % 64 == 0
+  int64_t k_half;        // k of one half of an operand read across its rows (K where there is one)
   void* y;               // [M][N], ld ldy (nullptr: only pre)
   void* y2;              // rows >= y_rows of the result go to y2 (weight gradients of two weights)
-  int64_t ldy, y_rows;
+  int64_t ldy, y_rows, y_valid;  // of each half's rows, y_valid are written
   const void* bias;      // [N], of the output's type; bias2: of the second half
   const void* bias2;
-  const void* res;       // [M][N], ld ldr
+  const void* res;       // [M][N], ld ldr; the backward epilogues: dy
   int64_t ldr;
-  float* pre;            // [M][halves * N] fp32, before the activation
+  float* pre;            // [M][halves][n8] fp32, before the activation
   float* slab;           // split-k partial sums [splits][M][N]
+  uint16_t* rows;        // backward epilogues: the gradient before the activation, planes of [M][halves * np]
+  int64_t rows_plane;
+  float* sums;           // backward epilogues, nullable: column sums [tiles of rows * WGM][halves * N]
+  int64_t n8, np;        // N rounded up to 8, to 64
   int32_t act, splits, vec;
 };
 
-enum Epi : int { kPlain = 0, kGated = 1, kSlab = 2 };
+// kDenseGrad / kGatedGrad: the product is the forward's, computed again; what leaves the kernel is the gradient
+// before the activation, dP = dy act'(p) or [dG | dU]
+enum Epi : int { kPlain = 0, kGated = 1, kSlab = 2, kDenseGrad = 3, kGatedGrad = 4 };
+// the operands read across their rows: none (forward), b (dx), both (dW)
+enum Across : int { kNone = 0, kB = 1, kBoth = 2 };
 
 template <int PA_, int PB_, int TM_, int TN_, int WGM_, int WGN_, int BK_>
 struct Config {
@@ -92,10 +105,30 @@ __device__ __forceinline__ int swz(int r, int c) {
   return U == 8 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3));
 }
 
+// Across the rows, LDS holds [k][rows]: 32-byte blocks of 16 rows, permuted by k so that the 16 values of k that one
+// transposing read touches (4 groups of 8, 4 of each) lie in different banks.
+template <int ROWS>
+__device__ __forceinline__ int swz_t(int k, int block) {
+  return block ^ (((k & 3) | ((k >> 3) << 2)) & (ROWS / 16 - 1));
+}
+
 __device__ __forceinline__ float act_fast(int kind, float v) {
   // hardware exp2 and reciprocal (about 2^-21): for results that are rounded to 8 bits
   if (kind == ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
   return act_fwd(kind, v);
+}
+
+// a(v) and a'(v)
+template <bool FAST>
+__device__ __forceinline__ void act_both(int kind, float v, float& a, float& da) {
+  if (FAST && kind == ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+    a = v * s;
+    da = s * (1.f + v * (1.f - s));
+  } else {
+    a = act_fwd(kind, v);
+    da = act_grad(kind, v);
+  }
 }
 
 template <typename T>
@@ -144,19 +177,104 @@ __device__ __forceinline__ void store4(T* p, floatx4 v, bool vec, int64_t left) 
   }
 }
 
-// One workgroup: one TM x TN tile (kGated: TN / 2 columns of each half) over one k range. Operands go
-// straight from global memory into LDS (16 bytes a lane, no registers), two stages: stage t + 1 is in flight
-// through the matrix work of stage t. The weight is the instruction's first operand, so that a lane holds
-// four consecutive columns of one row: 8- and 16-byte stores.
-template <typename C, int EPI, typename T>
+// Loads of one operand's stage into LDS, straight from global memory (16 bytes a lane, no registers).
+template <typename C, bool T, int P, int ROWS, int HALVES, int WT>
+struct Loader {
+  static constexpr int kWaves = C::kThreads / kWave;
+  static constexpr int kLoads = ROWS * C::U / kWave / kWaves;  // of a wave, per plane
+  static_assert(ROWS * C::U % (kWave * kWaves) == 0, "every wave issues whole loads");
+  static_assert(T || WT / HALVES >= C::kRowsPerLoad, "a load lies inside one half");
+  const Operand& o;
+  int64_t row0;
+  int wave, lane;
+  __amdgpu_buffer_rsrc_t r[T ? 1 : P][HALVES];
+
+  __device__ __forceinline__ Loader(const Operand& o_, int64_t row0_, int wave_, int lane_)
+      : o(o_), row0(row0_), wave(wave_), lane(lane_) {
+    if constexpr (!T) {  // one descriptor per plane and half, over the tile's rows
+      const int64_t left = o.rows - row0;
+      const uint32_t bytes = (uint32_t)(min((int64_t)(ROWS / HALVES), max(left, (int64_t)0)) * o.ld * 2);
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        r[q][0] = buffer_rsrc(o.p + q * o.plane + row0 * o.ld, bytes);
+        if (HALVES == 2) r[q][HALVES - 1] = buffer_rsrc(o.p2 + q * o.plane + row0 * o.ld, bytes);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load(char* base, int64_t step, int64_t k_half) const {
+    typedef __attribute__((address_space(3))) void lds_void;
+    if constexpr (T) {
+      constexpr int UR = ROWS / 8;  // units of a k row
+      int64_t k0 = step * C::BK;
+      const uint16_t* p = o.p;
+      if (k0 >= k_half) p = o.p2, k0 -= k_half;
+      // the descriptor of these k rows ends with the matrix
+      const int64_t kr = min((int64_t)C::BK, o.rows - k0);
+      const uint32_t bytes = kr > 0 && row0 < o.cols ? (uint32_t)(((kr - 1) * o.ld + o.cols - row0) * 2) : 0;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const __amdgpu_buffer_rsrc_t d = buffer_rsrc(p + q * o.plane + k0 * o.ld + row0, bytes);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int u0 = (j * kWaves + wave) * kWave, u = u0 + lane, k = u / UR, c = u % UR;
+          const uint32_t off = (uint32_t)k * (uint32_t)o.ld * 2 + swz_t<ROWS>(k, c >> 1) * 32 + (c & 1) * 16;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void*)(base + (q * ROWS * C::U + u0) * 16), 16, off, 0, 0, 0);
+        }
+      }
+    } else {
+      const uint32_t kb = (uint32_t)(step * C::BK * 2);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int u0 = (j * kWaves + wave) * kWave, r0 = u0 / C::U, row = r0 + lane / C::U;
+        // LDS row -> row of a half: a wave's WT columns are WT / 2 of the first half, then of the second
+        int src = row, half = 0;
+        if (HALVES == 2) {
+          constexpr int WH = WT / 2;
+          half = (r0 / WH) & 1;
+          src = row / WT * WH + row % WH;
+        }
+        const uint32_t off = (uint32_t)src * (uint32_t)o.ld * 2 + swz<C::U>(row, lane % C::U) * 16;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          lds_void* dst = (lds_void*)(base + (q * ROWS * C::U + u0) * 16);
+          if (HALVES == 1 || half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, off, kb, 0, 0);
+          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, off, kb, 0, 0);
+        }
+      }
+    }
+  }
+
+  // the fragment of 16 rows from `row` at k = kk * 32 .. + 31: lane = row % 16, 8 values of k from 8 (lane / 16)
+  static __device__ __forceinline__ bf16x8 fragment(const char* base, int q, int row, int kk, int lane) {
+    if constexpr (T) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      s16x4 h[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = kk * 32 + (lane >> 4) * 8 + i * 4 + ((lane & 15) >> 2);
+        const char* at = base + ((q * C::BK + k) * (ROWS / 8) + swz_t<ROWS>(k, row >> 4) * 2) * 16 + (lane & 3) * 8;
+        h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+      }
+      const s16x8 v = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(bf16x8, v);
+    } else {
+      const int r = row + (lane & 15);
+      return *reinterpret_cast<const bf16x8*>(base + ((q * ROWS + r) * C::U + swz<C::U>(r, kk * 4 + (lane >> 4))) * 16);
+    }
+  }
+};
+
+// One workgroup: one TM x TN tile (gated: TN / 2 columns of each half) over one k range. Two LDS stages: stage t + 1 is
+// in flight through the matrix work of stage t. The weight is the instruction's first operand, so that a lane
+// holds four consecutive columns of one row: 8- and 16-byte stores.
+template <typename C, int EPI, int ACROSS, typename T>
 __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const int tiles_m, const int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass drops the stub of a body with the LDS load builtin
-  constexpr int PA = C::PA, PB = C::PB, TM = C::TM, TN = C::TN, BK = C::BK, U = C::U;
-  constexpr int kHalves = EPI == kGated ? 2 : 1, TC = TN / kHalves;  // columns of a half in a tile
-  constexpr int kALoads = TM / C::kRowsPerLoad, kBLoads = TN / C::kRowsPerLoad;
-  constexpr int kWaves = C::kThreads / kWave;
-  static_assert(kALoads % kWaves == 0 && kBLoads % kWaves == 0, "every wave issues whole loads");
-  static_assert(C::WTN / kHalves >= C::kRowsPerLoad, "a load lies inside one half");
+  constexpr int PA = C::PA, PB = C::PB, TM = C::TM, TN = C::TN, BK = C::BK;
+  constexpr int kHalves = EPI == kGated || EPI == kGatedGrad ? 2 : 1, TC = TN / kHalves;  // columns of a half in a tile
+  static_assert(kHalves == 1 || ACROSS == kNone, "the gated epilogues belong to the forward product");
   __shared__ __attribute__((aligned(1024))) char lds[2 * C::kStage];
 
   // Workgroups go to the 8 XCDs in turn: give each XCD a contiguous run of tiles, so that neighbours share
@@ -170,7 +288,8 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
   constexpr int kGroup = 8;
   const int group = pid / (kGroup * tiles_n), first = group * kGroup;
   const int gsz = min(tiles_m - first, kGroup), in = pid - group * kGroup * tiles_n;
-  const int64_t m0 = (int64_t)(first + in % gsz) * TM, n0 = (int64_t)(in / gsz) * TC;
+  const int tm = first + in % gsz;
+  const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)(in / gsz) * TC;
 
   const int split = blockIdx.y;
   const int64_t steps = p.K / BK;
@@ -178,62 +297,10 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WGN, wn = wave % C::WGN;
-
-  // Descriptors: one per plane, over the tile's rows from its first k
-  __amdgpu_buffer_rsrc_t ra[PA], rb[PB][kHalves];
-  {
-    const int64_t left = p.a.rows - m0;
-    const uint32_t bytes = (uint32_t)(min((int64_t)TM, max(left, (int64_t)0)) * p.a.ld * 2);
-#pragma unroll
-    for (int q = 0; q < PA; ++q) ra[q] = buffer_rsrc(p.a.p + q * p.a.plane + m0 * p.a.ld, bytes);
-  }
-  {
-    const int64_t left = p.b.rows - n0;
-    const uint32_t bytes = (uint32_t)(min((int64_t)TC, max(left, (int64_t)0)) * p.b.ld * 2);
-#pragma unroll
-    for (int q = 0; q < PB; ++q) {
-      rb[q][0] = buffer_rsrc(p.b.p + q * p.b.plane + n0 * p.b.ld, bytes);
-      if (kHalves == 2) rb[q][kHalves - 1] = buffer_rsrc(p.b.p2 + q * p.b.plane + n0 * p.b.ld, bytes);
-    }
-  }
-  const int lr = lane / U, lu = lane % U;  // the row and unit of this lane in a load
-  const uint32_t lda2 = (uint32_t)p.a.ld * 2, ldb2 = (uint32_t)p.b.ld * 2;
-
-  auto load_stage = [&](int64_t step, int buf) {
-    const uint32_t kb = (uint32_t)(step * BK * 2);
-    char* base = lds + buf * C::kStage;
-#pragma unroll
-    for (int j = 0; j < kALoads / kWaves; ++j) {
-      const int row = (j * kWaves + wave) * C::kRowsPerLoad + lr;
-      const uint32_t off = (uint32_t)row * lda2 + swz<U>(row, lu) * 16;
-#pragma unroll
-      for (int q = 0; q < PA; ++q)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            ra[q], (__attribute__((address_space(3))) void*)(base + (q * TM * U + (j * kWaves + wave) * kWave) * 16), 16,
-            off, kb, 0, 0);
-    }
-    base += PA * TM * BK * 2;
-#pragma unroll
-    for (int j = 0; j < kBLoads / kWaves; ++j) {
-      const int r0 = (j * kWaves + wave) * C::kRowsPerLoad, row = r0 + lr;
-      // LDS row -> row of a half: a wave's WTN columns are WTN / 2 of the first half, then of the second
-      int src = row, half = 0;
-      if (kHalves == 2) {
-        constexpr int WH = C::WTN / 2;
-        half = (r0 / WH) & 1;
-        src = row / C::WTN * WH + row % WH;
-      }
-      const uint32_t off = (uint32_t)src * ldb2 + swz<U>(row, lu) * 16;
-#pragma unroll
-      for (int q = 0; q < PB; ++q) {
-        auto dst = (__attribute__((address_space(3))) void*)(base + (q * TN * U + (j * kWaves + wave) * kWave) * 16);
-        if (kHalves == 1 || half == 0)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rb[q][0], dst, 16, off, kb, 0, 0);
-        else
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rb[q][kHalves - 1], dst, 16, off, kb, 0, 0);
-      }
-    }
-  };
+  using LA = Loader<C, ACROSS == kBoth, PA, TM, 1, C::WTM>;
+  using LB = Loader<C, ACROSS != kNone, PB, TN, kHalves, C::WTN>;
+  const LA la(p.a, m0, wave, lane);
+  const LB lb(p.b, n0, wave, lane);
 
   floatx4 acc[C::FN][C::FM];
 #pragma unroll
@@ -241,7 +308,11 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 #pragma unroll
     for (int j = 0; j < C::FM; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int fr = lane & 15, fc = lane >> 4;  // fragment row, k unit
+  auto load_stage = [&](int64_t step, int buf) {
+    char* base = lds + buf * C::kStage;
+    la.load(base, step, p.k_half);
+    lb.load(base + PA * TM * BK * 2, step, p.k_half);
+  };
   if (s0 < s1) load_stage(s0, 0);
   for (int64_t s = s0; s < s1; ++s) {
     const int buf = (int)(s - s0) & 1;
@@ -258,17 +329,11 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 #pragma unroll
       for (int q = 0; q < PB; ++q)
 #pragma unroll
-        for (int i = 0; i < C::FN; ++i) {
-          const int r = wn * C::WTN + i * 16 + fr;
-          fb[q][i] = *reinterpret_cast<const bf16x8*>(sb + ((q * TN + r) * U + swz<U>(r, kk * 4 + fc)) * 16);
-        }
+        for (int i = 0; i < C::FN; ++i) fb[q][i] = LB::fragment(sb, q, wn * C::WTN + i * 16, kk, lane);
 #pragma unroll
       for (int q = 0; q < PA; ++q)
 #pragma unroll
-        for (int j = 0; j < C::FM; ++j) {
-          const int r = wm * C::WTM + j * 16 + fr;
-          fa[q][j] = *reinterpret_cast<const bf16x8*>(sa + ((q * TM + r) * U + swz<U>(r, kk * 4 + fc)) * 16);
-        }
+        for (int j = 0; j < C::FM; ++j) fa[q][j] = LA::fragment(sa, q, wm * C::WTM + j * 16, kk, lane);
       // small plane products first
 #pragma unroll
       for (int sum = (PA == 3 || PB == 3) ? 2 : 0; sum >= 0; --sum)
@@ -287,44 +352,106 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 
   // ------------------------------------------------------------------------------------------
   constexpr int FH = C::FN / kHalves;
+  constexpr bool kFast = sizeof(T) == 2;
+  const int fr = lane & 15, fc = lane >> 4;
   const bool vec = p.vec;
-#pragma unroll
-  for (int j = 0; j < C::FM; ++j) {
-    const int64_t m = m0 + wm * C::WTM + j * 16 + fr;
-    if (m >= p.M) continue;
+  if constexpr (EPI == kDenseGrad || EPI == kGatedGrad) {
+    constexpr int PL = sizeof(T) == 4 && PB == 3 ? 3 : 1;
 #pragma unroll
     for (int i = 0; i < FH; ++i) {
-      const int64_t n = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4;
-      if (n >= p.N) continue;
-      const int64_t left = p.N - n;
+      const int64_t n = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4, left = p.N - n;
       const bool v4 = vec && left >= 4;
-      floatx4 v = acc[i][j];
-      if constexpr (EPI == kSlab) {
-        store4(p.slab + ((int64_t)split * p.M + m) * p.N + n, v, v4, left);
-      } else if constexpr (EPI == kGated) {
-        floatx4 u = acc[i + FH][j];
-        if (p.bias) v += load4((const T*)p.bias + n, v4, left);
-        if (p.bias2) u += load4((const T*)p.bias2 + n, v4, left);
-        if (p.pre) {
-          store4(p.pre + m * 2 * p.N + n, v, v4, left);
-          store4(p.pre + m * 2 * p.N + p.N + n, u, v4, left);
-        }
-        if (p.y) {
+      floatx4 total[kHalves];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (sizeof(T) == 2 ? act_fast(p.act, v[e]) : act_fwd(p.act, v[e])) * u[e];
-          store4((T*)p.y + m * p.ldy + n, v, v4, left);
+      for (int h = 0; h < kHalves; ++h) total[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+      floatx4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
+      if (p.bias) b0 = load4((const T*)p.bias + n, v4, left);
+      if (kHalves == 2 && p.bias2) b1 = load4((const T*)p.bias2 + n, v4, left);
+#pragma unroll
+      for (int j = 0; j < C::FM; ++j) {
+        const int64_t m = m0 + wm * C::WTM + j * 16 + fr;
+        if (m >= p.M || n >= p.np) continue;
+        const floatx4 d = load4((const T*)p.res + m * p.ldr + n, v4, left);
+        floatx4 v = acc[i][j] + b0, out[kHalves];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float a, da;
+          act_both<kFast>(p.act, v[e], a, da);
+          if constexpr (kHalves == 2) {
+            const float u = acc[i + FH][j][e] + b1[e];
+            out[0][e] = d[e] * u * da;
+            out[kHalves - 1][e] = d[e] * a;
+          } else {
+            out[0][e] = d[e] * da;
+          }
         }
-      } else {
-        if (p.bias) v += load4((const T*)p.bias + n, v4, left);
-        if (p.pre) store4(p.pre + m * p.N + n, v, v4, left);
-        if (p.y) {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          total[h] += out[h];
+          u16x4 o[PL];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (PL == 1) {
+              o[0][e] = to_bf16(out[h][e]);
+            } else {
+              uint16_t q3[3];
+              split3(out[h][e], q3);
+#pragma unroll
+              for (int q = 0; q < 3; ++q) o[q][e] = q3[q];
+            }
+          }
+          uint16_t* at = p.rows + m * kHalves * p.np + h * p.np + n;
+#pragma unroll
+          for (int q = 0; q < PL; ++q) *reinterpret_cast<u16x4*>(at + q * p.rows_plane) = o[q];
+        }
+      }
+      if (p.sums) {  // the 16 rows of a fragment in a fixed tree
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float t = total[h][e];
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o);
+            if (fr == 0 && e < left) p.sums[((int64_t)tm * C::WGM + wm) * kHalves * p.N + h * p.N + n + e] = t;
+          }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < C::FM; ++j) {
+      const int64_t m = m0 + wm * C::WTM + j * 16 + fr;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int i = 0; i < FH; ++i) {
+        const int64_t n = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4;
+        if (n >= p.N) continue;
+        const int64_t left = p.N - n;
+        const bool v4 = vec && left >= 4;
+        floatx4 v = acc[i][j];
+        if constexpr (EPI == kSlab) {
+          store4(p.slab + ((int64_t)split * p.M + m) * p.N + n, v, v4, left);
+        } else if constexpr (EPI == kGated) {
+          floatx4 u = acc[i + FH][j];
+          if (p.bias) v += load4((const T*)p.bias + n, v4, left);
+          if (p.bias2) u += load4((const T*)p.bias2 + n, v4, left);
+          if (p.pre) {
+            *reinterpret_cast<floatx4*>(p.pre + m * 2 * p.n8 + n) = v;
+            *reinterpret_cast<floatx4*>(p.pre + m * 2 * p.n8 + p.n8 + n) = u;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (kFast ? act_fast(p.act, v[e]) : act_fwd(p.act, v[e])) * u[e];
+          store4((T*)p.y + m * p.ldy + n, v, v4, left);
+        } else {
+          if (p.bias) v += load4((const T*)p.bias + n, v4, left);
+          if (p.pre) *reinterpret_cast<floatx4*>(p.pre + m * p.n8 + n) = v;
           if (p.act >= 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = sizeof(T) == 2 ? act_fast(p.act, v[e]) : act_fwd(p.act, v[e]);
+            for (int e = 0; e < 4; ++e) v[e] = kFast ? act_fast(p.act, v[e]) : act_fwd(p.act, v[e]);
           }
           if (p.res) v += load4((const T*)p.res + m * p.ldr + n, v4, left);
-          T* y = m < p.y_rows ? (T*)p.y + m * p.ldy : (T*)p.y2 + (m - p.y_rows) * p.ldy;
-          store4(y + n, v, v4, left);
+          const int64_t r = m < p.y_rows ? m : m - p.y_rows;
+          if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, v, v4, left);
         }
       }
     }
@@ -335,24 +462,45 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 // A tile shape (0: the largest) and the number of k ranges of one launch.
 struct Plan {
   int tile, splits;
+  int waves_m;  // rows of waves of the tile, over tile_m rows: the column sums' parts are per wave row
+  int64_t tile_m;
 };
 // `columns`: of both halves together. may_split: a plain product whose partial sums may go to slabs.
 Plan plan_one(int64_t M, int64_t columns, int64_t K, bool may_split);
 Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split);
-// Launchers (dense_bf16.hip: one plane a side; dense_split.hip: three planes on one side or both, fp32 out).
-// p.splits > 1: the partial sums go to p.slab and reduce_slabs (dense.hip) applies the epilogue.
-int launch_one(const Problem& p, int tile, int halves, bool fp32_out, hipStream_t st);
-int launch_split(const Problem& p, int tile, int pa, int pb, int halves, hipStream_t st);
+// Launchers (dense_bf16.hip: one plane a side; dense_split.hip: three planes on one side or both, fp32 tensors).
+// epi: kPlain, kGated, kDenseGrad or kGatedGrad. p.splits > 1 (kPlain): the partial sums go to p.slab, and the
+// caller's reduction applies the epilogue.
+int launch_one(const Problem& p, int tile, int epi, int across, bool fp32, hipStream_t st);
+int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, hipStream_t st);
 
-template <typename C, int EPI, typename T>
+template <typename C, int EPI, int ACROSS, typename T>
 int launch_config(const Problem& p, hipStream_t st) {
-  constexpr int TC = C::TN / (EPI == kGated ? 2 : 1);
-  const int64_t tm = cdiv(p.M, C::TM), tn = cdiv(p.N, TC);
+  constexpr int TC = C::TN / (EPI == kGated || EPI == kGatedGrad ? 2 : 1);
+  // the backward epilogues write the padding behind column N too
+  const int64_t tm = cdiv(p.M, C::TM), tn = cdiv(EPI == kDenseGrad || EPI == kGatedGrad ? p.np : p.N, TC);
   if (tm * tn > (int64_t)INT32_MAX) return AIMX_EARG;
-  hipLaunchKernelGGL((k_dense<C, EPI, T>), dim3((unsigned)(tm * tn), (unsigned)p.splits), dim3(C::kThreads), 0, st, p,
-                     (int)tm, (int)tn);
+  hipLaunchKernelGGL((k_dense<C, EPI, ACROSS, T>), dim3((unsigned)(tm * tn), (unsigned)p.splits), dim3(C::kThreads), 0,
+                     st, p, (int)tm, (int)tn);
   AIMX_CHECK_LAUNCH();
   return AIMX_OK;
+}
+
+// the operand orders that occur with each epilogue
+template <typename C, typename T>
+int launch_epi(const Problem& p, int epi, int across, hipStream_t st) {
+  if (p.splits > 1) {
+    if (across == kNone) return launch_config<C, kSlab, kNone, float>(p, st);
+    return across == kB ? launch_config<C, kSlab, kB, float>(p, st) : launch_config<C, kSlab, kBoth, float>(p, st);
+  }
+  switch (epi) {
+    case kGated: return launch_config<C, kGated, kNone, T>(p, st);
+    case kDenseGrad: return launch_config<C, kDenseGrad, kNone, T>(p, st);
+    case kGatedGrad: return launch_config<C, kGatedGrad, kNone, T>(p, st);
+    default: break;
+  }
+  if (across == kNone) return launch_config<C, kPlain, kNone, T>(p, st);
+  return across == kB ? launch_config<C, kPlain, kB, T>(p, st) : launch_config<C, kPlain, kBoth, T>(p, st);
 }
 
 }  // namespace dense

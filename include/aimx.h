@@ -588,8 +588,10 @@ int aimx_pad_batch(const AimxPadBatch* p, aimx_stream_t stream);
  * precision: of fp32 tensors. AIMX_PREC_FP32: fp32 accuracy on the bf16 matrix cores (three exact bf16
  * parts per operand, six products); AIMX_PREC_BF16: operands rounded to bf16, everything else fp32.
  * Sums are fp32. An infinite operand of an AIMX_PREC_FP32 product may give NaN instead of an infinity.
- * pre (nullable, fp32 [M, halves * N], 16-byte aligned): the values before the activation, kept for
- * aimx_dense_backward; without them (act != none) the backward computes them again.
+ * pre (nullable, fp32 [M, halves, N rounded up to 8], 16-byte aligned): the values before the activation, kept for
+ * aimx_dense_backward; without them (act != none) the backward computes them again from x or its 8-bit
+ * form, which bf16 tensors do faster. An fp32 product (AIMX_PREC_FP32) from x itself keeps them: there
+ * pre must not be NULL in the backward.
  * The workspace (16-byte aligned, aimx_dense_workspace_bytes / aimx_dense_backward_workspace_bytes) holds
  * staged operands and partial sums. Sums over ranges of k and of rows are joined in a fixed order.
  * Row strides <= 2^21 elements, N, K <= 2^21; the backward takes M <= 2^22 rows.
