@@ -112,22 +112,38 @@ __device__ __forceinline__ int swz_t(int k, int block) {
   return block ^ (((k & 3) | ((k >> 3) << 2)) & (ROWS / 16 - 1));
 }
 
-__device__ __forceinline__ float act_fast(int kind, float v) {
-  // hardware exp2 and reciprocal (about 2^-21): for results that are rounded to 8 bits
-  if (kind == ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
-  return act_fwd(kind, v);
-}
-
-// a(v) and a'(v)
-template <bool FAST>
-__device__ __forceinline__ void act_both(int kind, float v, float& a, float& da) {
-  if (FAST && kind == ACT_SILU) {
+// Activations of several values with one branch on the kind: a branch per value costs more than the value's
+// arithmetic. FAST: hardware exp2 and reciprocal (about 2^-21 each) in silu, for results rounded to 8 bits.
+template <bool FAST, int KIND>
+__device__ __forceinline__ void act_one(float v, float& a, float& da) {
+  if constexpr (FAST && KIND == ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
     a = v * s;
     da = s * (1.f + v * (1.f - s));
+  } else if constexpr (KIND == ACT_SILU) {
+    const float s = 1.f / (1.f + expf(-v));
+    a = v / (1.f + expf(-v));
+    da = s * (1.f + v * (1.f - s));
   } else {
-    a = act_fwd(kind, v);
-    da = act_grad(kind, v);
+    a = act_fwd(KIND, v);
+    da = act_grad(KIND, v);
+  }
+}
+template <bool FAST, int KIND, int N>
+__device__ __forceinline__ void act_each(const float (&v)[N], float (&a)[N], float (&da)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) act_one<FAST, KIND>(v[i], a[i], da[i]);
+}
+// a(v) and a'(v); what the caller does not use is not computed
+template <bool FAST, int N>
+__device__ __forceinline__ void act_all(int kind, const float (&v)[N], float (&a)[N], float (&da)[N]) {
+  switch (kind) {
+    case ACT_RELU: return act_each<FAST, ACT_RELU>(v, a, da);
+    case ACT_LEAKYRELU: return act_each<FAST, ACT_LEAKYRELU>(v, a, da);
+    case ACT_ELU: return act_each<FAST, ACT_ELU>(v, a, da);
+    case ACT_GELU: return act_each<FAST, ACT_GELU>(v, a, da);
+    case ACT_SILU: return act_each<FAST, ACT_SILU>(v, a, da);
+    default: return act_each<FAST, ACT_NONE>(v, a, da);
   }
 }
 
@@ -156,6 +172,28 @@ __device__ __forceinline__ floatx4 load4(const T* p, bool vec, int64_t left) {
   }
   return v;
 }
+// the same as loaded, converted where it is used
+template <typename T>
+struct Raw4 {
+  floatx4 f;
+  __device__ __forceinline__ void load(const T* p, bool vec, int64_t left) { f = load4(p, vec, left); }
+  __device__ __forceinline__ floatx4 get() const { return f; }
+};
+template <>
+struct Raw4<uint16_t> {
+  u16x4 h;
+  __device__ __forceinline__ void load(const uint16_t* p, bool vec, int64_t left) {
+    if (vec) {
+      h = *reinterpret_cast<const u16x4*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = i < left ? p[i] : (uint16_t)0;
+    }
+  }
+  __device__ __forceinline__ floatx4 get() const {
+    return floatx4{from_bf16(h[0]), from_bf16(h[1]), from_bf16(h[2]), from_bf16(h[3])};
+  }
+};
 template <typename T>
 __device__ __forceinline__ void store4(T* p, floatx4 v, bool vec, int64_t left) {
   if (vec) {
@@ -175,6 +213,43 @@ __device__ __forceinline__ void store4(T* p, floatx4 v, bool vec, int64_t left) 
         else p[i] = to_bf16(v[i]);
       }
   }
+}
+
+// Transposing reads of F fragments, the two halves of each OFF bytes apart, and the wait for them in one block: behind
+// the builtin the compiler waits for every load into LDS in flight, the next stage's too (it cannot tell
+// them apart), which took a third of the product's rate.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+#define AIMX_TR(o, a) "ds_read_b64_tr_b16 %" #o ", %" #a "\n\t"
+#define AIMX_TR2(o, a, n) "ds_read_b64_tr_b16 %" #o ", %" #a " offset:%" #n "\n\t"
+template <int OFF>
+__device__ __forceinline__ void read_t2(const uint32_t* a, s16x4* l, s16x4* h) {
+  asm volatile(AIMX_TR(0, 4) AIMX_TR(1, 5) AIMX_TR2(2, 4, 6) AIMX_TR2(3, 5, 6) "s_waitcnt lgkmcnt(0)"
+               : "=&v"(l[0]), "=&v"(l[1]), "=&v"(h[0]), "=&v"(h[1])
+               : "v"(a[0]), "v"(a[1]), "n"(OFF)
+               : "memory");
+}
+template <int OFF>
+__device__ __forceinline__ void read_t4(const uint32_t* a, s16x4* l, s16x4* h) {
+  asm volatile(AIMX_TR(0, 8) AIMX_TR2(4, 8, 12) AIMX_TR(1, 9) AIMX_TR2(5, 9, 12) AIMX_TR(2, 10) AIMX_TR2(6, 10, 12)
+                   AIMX_TR(3, 11) AIMX_TR2(7, 11, 12) "s_waitcnt lgkmcnt(0)"
+               : "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3])
+               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
+               : "memory");
+}
+template <int OFF, int F>
+__device__ __forceinline__ void read_t(const uint32_t (&at)[F], bf16x8 (&f)[F]) {
+  s16x4 l[F], h[F];
+  static_assert(F == 2 || F % 4 == 0, "");
+  if constexpr (F == 2) {
+    read_t2<OFF>(at, l, h);
+  } else {
+#pragma unroll
+    for (int j = 0; j < F; j += 4) read_t4<OFF>(at + j, l + j, h + j);
+  }
+#pragma unroll
+  for (int j = 0; j < F; ++j)
+    f[j] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(l[j], h[j], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // Loads of one operand's stage into LDS, straight from global memory (16 bytes a lane, no registers).
@@ -245,26 +320,160 @@ struct Loader {
     }
   }
 
-  // the fragment of 16 rows from `row` at k = kk * 32 .. + 31: lane = row % 16, 8 values of k from 8 (lane / 16)
-  static __device__ __forceinline__ bf16x8 fragment(const char* base, int q, int row, int kk, int lane) {
+  // Fragments of 16 rows, F of them from row `row`, at k = kk * 32 .. + 31: lane = row % 16, 8 values of k from
+  // 8 (lane / 16) on.
+  template <int F>
+  static __device__ __forceinline__ void fragments(const char* base, int q, int row, int kk, int lane, bf16x8 (&f)[F]) {
     if constexpr (T) {
-      typedef short s16x4 __attribute__((ext_vector_type(4)));
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
-      s16x4 h[2];
+      // k = kk * 32 + 8 (lane / 16) + 4 i + (lane % 16) / 4 for the halves i of the 8 values: the blocks'
+      // permutation depends on the lane alone
+      const int kl = (lane >> 4) * 8 + ((lane & 15) >> 2);
+      const uint32_t at0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)base +
+                           ((q * C::BK + kk * 32 + kl) * (ROWS / 8)) * 16 + (lane & 3) * 8;
+      uint32_t at[F];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int k = kk * 32 + (lane >> 4) * 8 + i * 4 + ((lane & 15) >> 2);
-        const char* at = base + ((q * C::BK + k) * (ROWS / 8) + swz_t<ROWS>(k, row >> 4) * 2) * 16 + (lane & 3) * 8;
-        h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-      }
-      const s16x8 v = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      return __builtin_bit_cast(bf16x8, v);
+      for (int j = 0; j < F; ++j) at[j] = at0 + swz_t<ROWS>(kl, (row >> 4) + j) * 32;
+      read_t<4 * ROWS * 2>(at, f);
     } else {
-      const int r = row + (lane & 15);
-      return *reinterpret_cast<const bf16x8*>(base + ((q * ROWS + r) * C::U + swz<C::U>(r, kk * 4 + (lane >> 4))) * 16);
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        const int r = row + j * 16 + (lane & 15);
+        f[j] = *reinterpret_cast<const bf16x8*>(base + ((q * ROWS + r) * C::U + swz<C::U>(r, kk * 4 + (lane >> 4))) * 16);
+      }
     }
   }
 };
+
+template <typename C, int EPI, typename T, bool VEC>
+__device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN][C::FM], int tm, int64_t m0, int64_t n0,
+                                         int wm, int wn, int lane, int split) {
+  constexpr int kHalves = EPI == kGated || EPI == kGatedGrad ? 2 : 1, FH = C::FN / kHalves;
+  constexpr bool kFast = sizeof(T) == 2, kGrad = EPI == kDenseGrad || EPI == kGatedGrad;
+  constexpr int PL = kGrad && sizeof(T) == 4 && C::PB == 3 ? 3 : 1;
+  const int fr = lane & 15, fc = lane >> 4;
+  int64_t nn[FH], nl[FH];  // a lane's first columns, where they are loaded from
+  floatx4 b0[FH], b1[FH], total[kHalves][FH];
+#pragma unroll
+  for (int i = 0; i < FH; ++i) {
+    nn[i] = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4;
+    nl[i] = VEC ? min(nn[i], p.N - 4) : nn[i];
+    b0[i] = b1[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (EPI != kSlab) {
+      if (p.bias) b0[i] = load4((const T*)p.bias + nl[i], VEC, p.N - nn[i]);
+      if (kHalves == 2 && p.bias2) b1[i] = load4((const T*)p.bias2 + nl[i], VEC, p.N - nn[i]);
+    }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) total[h][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr bool kRes = EPI == kPlain || kGrad;
+  // rows whose operands are in flight together, 16 registers of them
+  constexpr int kMost = 16 / sizeof(T) / FH, kAhead = kMost < 1 ? 1 : kMost < C::FM ? kMost : C::FM;
+#pragma unroll
+  for (int j0 = 0; j0 < C::FM; j0 += kAhead) {
+    Raw4<T> d[kAhead][FH];
+    if constexpr (kRes) {
+      if (p.res) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int64_t m = min(m0 + wm * C::WTM + (j0 + j) * 16 + fr, p.M - 1);
+#pragma unroll
+          for (int i = 0; i < FH; ++i) d[j][i].load((const T*)p.res + m * p.ldr + nl[i], VEC, p.N - nn[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int jj = 0; jj < kAhead; ++jj) {
+      const int j = j0 + jj;
+      const int64_t m = m0 + wm * C::WTM + j * 16 + fr;
+      if (m >= p.M) continue;
+      float v[FH * 4], a[FH * 4], da[FH * 4];
+#pragma unroll
+      for (int i = 0; i < FH; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[4 * i + e] = v[4 * i + e] = acc[i][j][e] + b0[i][e];
+      if constexpr (EPI == kGated || EPI == kPlain) {
+        if (p.pre) {
+#pragma unroll
+          for (int i = 0; i < FH; ++i) {
+            if (nn[i] >= p.N) continue;
+            float* at = p.pre + m * kHalves * p.n8 + nn[i];
+            *reinterpret_cast<floatx4*>(at) = floatx4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+            if constexpr (kHalves == 2) *reinterpret_cast<floatx4*>(at + p.n8) = acc[i + FH][j] + b1[i];
+          }
+        }
+      }
+      if constexpr (kGrad || EPI == kGated) {
+        act_all<kFast>(p.act, v, a, da);
+      } else if constexpr (EPI == kPlain) {
+        if (p.act >= 0) act_all<kFast>(p.act, v, a, da);
+      }
+#pragma unroll
+      for (int i = 0; i < FH; ++i) {
+        const int64_t n = nn[i], left = p.N - n;
+        if (n >= (kGrad ? p.np : p.N)) continue;
+        floatx4 o = {a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
+        if constexpr (kGrad) {
+          floatx4 out[kHalves];
+          const floatx4 dd = VEC && left <= 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : d[jj][i].get();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (kHalves == 2) {
+              out[0][e] = dd[e] * (acc[i + FH][j][e] + b1[i][e]) * da[4 * i + e];
+              out[kHalves - 1][e] = dd[e] * o[e];
+            } else {
+              out[0][e] = dd[e] * da[4 * i + e];
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            total[h][i] += out[h];
+            u16x4 w[PL];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (PL == 1) {
+                w[0][e] = to_bf16(out[h][e]);
+              } else {
+                uint16_t q3[3];
+                split3(out[h][e], q3);
+#pragma unroll
+                for (int q = 0; q < PL; ++q) w[q][e] = q3[q];
+              }
+            }
+            uint16_t* at = p.rows + (m * kHalves + h) * p.np + n;
+#pragma unroll
+            for (int q = 0; q < PL; ++q) *reinterpret_cast<u16x4*>(at + q * p.rows_plane) = w[q];
+          }
+        } else if constexpr (EPI == kSlab) {
+          store4(p.slab + ((int64_t)split * p.M + m) * p.N + n, o, VEC, left);
+        } else if constexpr (EPI == kGated) {
+          store4((T*)p.y + m * p.ldy + n, o * (acc[i + FH][j] + b1[i]), VEC, left);
+        } else {
+          if (p.res) o += d[jj][i].get();
+          const int64_t r = m < p.y_rows ? m : m - p.y_rows;
+          if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, o, VEC, left);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // or the addresses of every row are live at once
+  }
+  if constexpr (kGrad) {
+    if (p.sums) {  // the 16 rows of a fragment in a fixed tree
+#pragma unroll
+      for (int i = 0; i < FH; ++i)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float t = total[h][i][e];
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o);
+            if (fr == 0 && nn[i] + e < p.N)
+              p.sums[((int64_t)tm * C::WGM + wm) * kHalves * p.N + h * p.N + nn[i] + e] = t;
+          }
+    }
+  }
+}
 
 // One workgroup: one TM x TN tile (gated: TN / 2 columns of each half) over one k range. Two LDS stages: stage t + 1 is
 // in flight through the matrix work of stage t. The weight is the instruction's first operand, so that a lane
@@ -327,13 +536,9 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
     for (int kk = 0; kk < BK / 32; ++kk) {
       bf16x8 fa[PA][C::FM], fb[PB][C::FN];
 #pragma unroll
-      for (int q = 0; q < PB; ++q)
+      for (int q = 0; q < PB; ++q) LB::template fragments<C::FN>(sb, q, wn * C::WTN, kk, lane, fb[q]);
 #pragma unroll
-        for (int i = 0; i < C::FN; ++i) fb[q][i] = LB::fragment(sb, q, wn * C::WTN + i * 16, kk, lane);
-#pragma unroll
-      for (int q = 0; q < PA; ++q)
-#pragma unroll
-        for (int j = 0; j < C::FM; ++j) fa[q][j] = LA::fragment(sa, q, wm * C::WTM + j * 16, kk, lane);
+      for (int q = 0; q < PA; ++q) LA::template fragments<C::FM>(sa, q, wm * C::WTM, kk, lane, fa[q]);
       // small plane products first
 #pragma unroll
       for (int sum = (PA == 3 || PB == 3) ? 2 : 0; sum >= 0; --sum)
@@ -351,111 +556,10 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
   }
 
   // ------------------------------------------------------------------------------------------
-  constexpr int FH = C::FN / kHalves;
-  constexpr bool kFast = sizeof(T) == 2;
-  const int fr = lane & 15, fc = lane >> 4;
-  const bool vec = p.vec;
-  if constexpr (EPI == kDenseGrad || EPI == kGatedGrad) {
-    constexpr int PL = sizeof(T) == 4 && PB == 3 ? 3 : 1;
-#pragma unroll
-    for (int i = 0; i < FH; ++i) {
-      const int64_t n = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4, left = p.N - n;
-      const bool v4 = vec && left >= 4;
-      floatx4 total[kHalves];
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) total[h] = floatx4{0.f, 0.f, 0.f, 0.f};
-      floatx4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
-      if (p.bias) b0 = load4((const T*)p.bias + n, v4, left);
-      if (kHalves == 2 && p.bias2) b1 = load4((const T*)p.bias2 + n, v4, left);
-#pragma unroll
-      for (int j = 0; j < C::FM; ++j) {
-        const int64_t m = m0 + wm * C::WTM + j * 16 + fr;
-        if (m >= p.M || n >= p.np) continue;
-        const floatx4 d = load4((const T*)p.res + m * p.ldr + n, v4, left);
-        floatx4 v = acc[i][j] + b0, out[kHalves];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a, da;
-          act_both<kFast>(p.act, v[e], a, da);
-          if constexpr (kHalves == 2) {
-            const float u = acc[i + FH][j][e] + b1[e];
-            out[0][e] = d[e] * u * da;
-            out[kHalves - 1][e] = d[e] * a;
-          } else {
-            out[0][e] = d[e] * da;
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          total[h] += out[h];
-          u16x4 o[PL];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (PL == 1) {
-              o[0][e] = to_bf16(out[h][e]);
-            } else {
-              uint16_t q3[3];
-              split3(out[h][e], q3);
-#pragma unroll
-              for (int q = 0; q < 3; ++q) o[q][e] = q3[q];
-            }
-          }
-          uint16_t* at = p.rows + m * kHalves * p.np + h * p.np + n;
-#pragma unroll
-          for (int q = 0; q < PL; ++q) *reinterpret_cast<u16x4*>(at + q * p.rows_plane) = o[q];
-        }
-      }
-      if (p.sums) {  // the 16 rows of a fragment in a fixed tree
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float t = total[h][e];
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o);
-            if (fr == 0 && e < left) p.sums[((int64_t)tm * C::WGM + wm) * kHalves * p.N + h * p.N + n + e] = t;
-          }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < C::FM; ++j) {
-      const int64_t m = m0 + wm * C::WTM + j * 16 + fr;
-      if (m >= p.M) continue;
-#pragma unroll
-      for (int i = 0; i < FH; ++i) {
-        const int64_t n = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4;
-        if (n >= p.N) continue;
-        const int64_t left = p.N - n;
-        const bool v4 = vec && left >= 4;
-        floatx4 v = acc[i][j];
-        if constexpr (EPI == kSlab) {
-          store4(p.slab + ((int64_t)split * p.M + m) * p.N + n, v, v4, left);
-        } else if constexpr (EPI == kGated) {
-          floatx4 u = acc[i + FH][j];
-          if (p.bias) v += load4((const T*)p.bias + n, v4, left);
-          if (p.bias2) u += load4((const T*)p.bias2 + n, v4, left);
-          if (p.pre) {
-            *reinterpret_cast<floatx4*>(p.pre + m * 2 * p.n8 + n) = v;
-            *reinterpret_cast<floatx4*>(p.pre + m * 2 * p.n8 + p.n8 + n) = u;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (kFast ? act_fast(p.act, v[e]) : act_fwd(p.act, v[e])) * u[e];
-          store4((T*)p.y + m * p.ldy + n, v, v4, left);
-        } else {
-          if (p.bias) v += load4((const T*)p.bias + n, v4, left);
-          if (p.pre) *reinterpret_cast<floatx4*>(p.pre + m * p.n8 + n) = v;
-          if (p.act >= 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = kFast ? act_fast(p.act, v[e]) : act_fwd(p.act, v[e]);
-          }
-          if (p.res) v += load4((const T*)p.res + m * p.ldr + n, v4, left);
-          const int64_t r = m < p.y_rows ? m : m - p.y_rows;
-          if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, v, v4, left);
-        }
-      }
-    }
-  }
+  // Where every row starts at a multiple of four elements, the epilogue's operands come by unconditional loads
+  // (of the last row and columns in place of those past the end), all in flight together.
+  if (p.vec) epilogue<C, EPI, T, true>(p, acc, tm, m0, n0, wm, wn, lane, split);
+  else epilogue<C, EPI, T, false>(p, acc, tm, m0, n0, wm, wn, lane, split);
 #endif
 }
 
