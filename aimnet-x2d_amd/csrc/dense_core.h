@@ -105,11 +105,11 @@ __device__ __forceinline__ int swz(int r, int c) {
   return U == 8 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3));
 }
 
-// Across the rows, LDS holds [k][rows]: 32-byte blocks of 16 rows, permuted by k so that the 16 values of k that one
-// transposing read touches (4 groups of 8, 4 of each) lie in different banks.
+// Across the rows, LDS holds [k][rows]: 32-byte blocks of 16 rows, permuted by k so that the values of k that half a
+// wave's transposing read touches (2 groups of 8, 4 of each) lie in different banks.
 template <int ROWS>
 __device__ __forceinline__ int swz_t(int k, int block) {
-  return block ^ (((k & 3) | ((k >> 3) << 2)) & (ROWS / 16 - 1));
+  return block ^ (((k & 3) | ((k >> 1) & 4)) & (ROWS / 16 - 1));
 }
 
 // Activations of several values with one branch on the kind: a branch per value costs more than the value's
@@ -215,58 +215,43 @@ __device__ __forceinline__ void store4(T* p, floatx4 v, bool vec, int64_t left) 
   }
 }
 
-// Transposing reads of F fragments, the two halves of each OFF bytes apart, and the wait for them in one block: behind
-// the builtin the compiler waits for every load into LDS in flight, the next stage's too (it cannot tell
-// them apart), which took a third of the product's rate.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-#define AIMX_TR(o, a) "ds_read_b64_tr_b16 %" #o ", %" #a "\n\t"
-#define AIMX_TR2(o, a, n) "ds_read_b64_tr_b16 %" #o ", %" #a " offset:%" #n "\n\t"
-template <int OFF>
-__device__ __forceinline__ void read_t2(const uint32_t* a, s16x4* l, s16x4* h) {
-  asm volatile(AIMX_TR(0, 4) AIMX_TR(1, 5) AIMX_TR2(2, 4, 6) AIMX_TR2(3, 5, 6) "s_waitcnt lgkmcnt(0)"
-               : "=&v"(l[0]), "=&v"(l[1]), "=&v"(h[0]), "=&v"(h[1])
-               : "v"(a[0]), "v"(a[1]), "n"(OFF)
-               : "memory");
-}
-template <int OFF>
-__device__ __forceinline__ void read_t4(const uint32_t* a, s16x4* l, s16x4* h) {
-  asm volatile(AIMX_TR(0, 8) AIMX_TR2(4, 8, 12) AIMX_TR(1, 9) AIMX_TR2(5, 9, 12) AIMX_TR(2, 10) AIMX_TR2(6, 10, 12)
-                   AIMX_TR(3, 11) AIMX_TR2(7, 11, 12) "s_waitcnt lgkmcnt(0)"
-               : "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3])
-               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF)
-               : "memory");
-}
-template <int OFF, int F>
-__device__ __forceinline__ void read_t(const uint32_t (&at)[F], bf16x8 (&f)[F]) {
-  s16x4 l[F], h[F];
-  static_assert(F == 2 || F % 4 == 0, "");
-  if constexpr (F == 2) {
-    read_t2<OFF>(at, l, h);
-  } else {
-#pragma unroll
-    for (int j = 0; j < F; j += 4) read_t4<OFF>(at + j, l + j, h + j);
-  }
-#pragma unroll
-  for (int j = 0; j < F; ++j)
-    f[j] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(l[j], h[j], 0, 1, 2, 3, 4, 5, 6, 7));
-}
 
 // Loads of one operand's stage into LDS, straight from global memory (16 bytes a lane, no registers).
 template <typename C, bool T, int P, int ROWS, int HALVES, int WT>
 struct Loader {
   static constexpr int kWaves = C::kThreads / kWave;
   static constexpr int kLoads = ROWS * C::U / kWave / kWaves;  // of a wave, per plane
+  static constexpr int UR = ROWS / 8;                          // units of a k row, across
+  // rows (across: of k) that all waves' j-th loads cover: the permutations repeat after as many, so a lane has one
+  // offset and load j adds a scalar
+  static constexpr int kStep = kWaves * (T ? kWave / UR : C::kRowsPerLoad);
   static_assert(ROWS * C::U % (kWave * kWaves) == 0, "every wave issues whole loads");
-  static_assert(T || WT / HALVES >= C::kRowsPerLoad, "a load lies inside one half");
+  static_assert(kStep % (T ? 16 : 8) == 0, "the permutations repeat");
+  static_assert(T || HALVES == 1 || ((kStep % WT == 0 || WT / 2 % kStep == 0) && WT / 2 >= C::kRowsPerLoad),
+                "a load lies inside one half");
   const Operand& o;
   int64_t row0;
-  int wave, lane;
+  int wave;
+  uint32_t off;  // of this lane in load 0
   __amdgpu_buffer_rsrc_t r[T ? 1 : P][HALVES];
 
-  __device__ __forceinline__ Loader(const Operand& o_, int64_t row0_, int wave_, int lane_)
-      : o(o_), row0(row0_), wave(wave_), lane(lane_) {
-    if constexpr (!T) {  // one descriptor per plane and half, over the tile's rows
+  // the row of a half (gated: a wave's WT columns are WT / 2 of the first half, then of the second) that LDS row
+  // `row` holds
+  static __device__ __forceinline__ constexpr int source_row(int row) {
+    return HALVES == 1 ? row : row / WT * (WT / 2) + row % (WT / 2);
+  }
+
+  __device__ __forceinline__ Loader(const Operand& o_, int64_t row0_, int wave_, int lane) : o(o_), row0(row0_), wave(wave_) {
+    const int u = wave * kWave + lane;
+    if constexpr (T) {
+      const int k = u / UR, c = u % UR;
+      off = (uint32_t)k * (uint32_t)o.ld * 2 + swz_t<ROWS>(k, c >> 1) * 32 + (c & 1) * 16;
+    } else {
+      const int row = u / C::U;
+      off = (uint32_t)source_row(row) * (uint32_t)o.ld * 2 + swz<C::U>(row, u % C::U) * 16;
+      // one descriptor per plane and half, over the tile's rows
       const int64_t left = o.rows - row0;
       const uint32_t bytes = (uint32_t)(min((int64_t)(ROWS / HALVES), max(left, (int64_t)0)) * o.ld * 2);
 #pragma unroll
@@ -279,8 +264,8 @@ struct Loader {
 
   __device__ __forceinline__ void load(char* base, int64_t step, int64_t k_half) const {
     typedef __attribute__((address_space(3))) void lds_void;
+    const uint32_t ld2 = (uint32_t)o.ld * 2;
     if constexpr (T) {
-      constexpr int UR = ROWS / 8;  // units of a k row
       int64_t k0 = step * C::BK;
       const uint16_t* p = o.p;
       if (k0 >= k_half) p = o.p2, k0 -= k_half;
@@ -291,30 +276,21 @@ struct Loader {
       for (int q = 0; q < P; ++q) {
         const __amdgpu_buffer_rsrc_t d = buffer_rsrc(p + q * o.plane + k0 * o.ld + row0, bytes);
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          const int u0 = (j * kWaves + wave) * kWave, u = u0 + lane, k = u / UR, c = u % UR;
-          const uint32_t off = (uint32_t)k * (uint32_t)o.ld * 2 + swz_t<ROWS>(k, c >> 1) * 32 + (c & 1) * 16;
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lds_void*)(base + (q * ROWS * C::U + u0) * 16), 16, off, 0, 0, 0);
-        }
+        for (int j = 0; j < kLoads; ++j)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              d, (lds_void*)(base + (q * ROWS * C::U + (j * kWaves + wave) * kWave) * 16), 16, off, j * kStep * ld2, 0, 0);
       }
     } else {
       const uint32_t kb = (uint32_t)(step * C::BK * 2);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int u0 = (j * kWaves + wave) * kWave, r0 = u0 / C::U, row = r0 + lane / C::U;
-        // LDS row -> row of a half: a wave's WT columns are WT / 2 of the first half, then of the second
-        int src = row, half = 0;
-        if (HALVES == 2) {
-          constexpr int WH = WT / 2;
-          half = (r0 / WH) & 1;
-          src = row / WT * WH + row % WH;
-        }
-        const uint32_t off = (uint32_t)src * (uint32_t)o.ld * 2 + swz<C::U>(row, lane % C::U) * 16;
+        const int half = HALVES == 1 ? 0 : ((j * kStep + wave * C::kRowsPerLoad) / (WT / 2)) & 1;
+        const uint32_t at = kb + source_row(j * kStep) * ld2;
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          lds_void* dst = (lds_void*)(base + (q * ROWS * C::U + u0) * 16);
-          if (HALVES == 1 || half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, off, kb, 0, 0);
-          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, off, kb, 0, 0);
+          lds_void* dst = (lds_void*)(base + (q * ROWS * C::U + (j * kWaves + wave) * kWave) * 16);
+          if (half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, off, at, 0, 0);
+          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, off, at, 0, 0);
         }
       }
     }
@@ -328,12 +304,13 @@ struct Loader {
       // k = kk * 32 + 8 (lane / 16) + 4 i + (lane % 16) / 4 for the halves i of the 8 values: the blocks'
       // permutation depends on the lane alone
       const int kl = (lane >> 4) * 8 + ((lane & 15) >> 2);
-      const uint32_t at0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)base +
-                           ((q * C::BK + kk * 32 + kl) * (ROWS / 8)) * 16 + (lane & 3) * 8;
-      uint32_t at[F];
+      const char* at0 = base + ((q * C::BK + kk * 32 + kl) * (ROWS / 8)) * 16 + (lane & 3) * 8;
 #pragma unroll
-      for (int j = 0; j < F; ++j) at[j] = at0 + swz_t<ROWS>(kl, (row >> 4) + j) * 32;
-      read_t<4 * ROWS * 2>(at, f);
+      for (int j = 0; j < F; ++j) {
+        auto at = (__attribute__((address_space(3))) s16x4*)(at0 + swz_t<ROWS>(kl, (row >> 4) + j) * 32);
+        const s16x4 l = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at), h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + ROWS);
+        f[j] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < F; ++j) {
@@ -517,28 +494,22 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 #pragma unroll
     for (int j = 0; j < C::FM; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  auto load_stage = [&](int64_t step, int buf) {
-    char* base = lds + buf * C::kStage;
-    la.load(base, step, p.k_half);
-    lb.load(base + PA * TM * BK * 2, step, p.k_half);
+  // One stage: its fragments and their products, while the next stage comes in. The addresses are __restrict:
+  // without it the compiler takes every transposing read to depend on the loads into LDS in flight and waits
+  // for them first.
+  auto load = [&](char* at, int64_t step) __attribute__((always_inline)) {
+    la.load(at, step, p.k_half);
+    lb.load(at + PA * TM * BK * 2, step, p.k_half);
   };
-  if (s0 < s1) load_stage(s0, 0);
-  for (int64_t s = s0; s < s1; ++s) {
-    const int buf = (int)(s - s0) & 1;
-    // this wave's loads of stage s are in LDS; after the barrier everyone's are, and nobody reads the
-    // other buffer any more
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (s + 1 < s1) load_stage(s + 1, buf ^ 1);
-    const char* sa = lds + buf * C::kStage;
-    const char* sb = sa + PA * TM * BK * 2;
+  auto stage = [&](char* __restrict next, const char* __restrict now, int64_t s) __attribute__((always_inline)) {
+    if (s + 1 < s1) load(next, s + 1);
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
       bf16x8 fa[PA][C::FM], fb[PB][C::FN];
 #pragma unroll
-      for (int q = 0; q < PB; ++q) LB::template fragments<C::FN>(sb, q, wn * C::WTN, kk, lane, fb[q]);
+      for (int q = 0; q < PB; ++q) LB::template fragments<C::FN>(now + PA * TM * BK * 2, q, wn * C::WTN, kk, lane, fb[q]);
 #pragma unroll
-      for (int q = 0; q < PA; ++q) LA::template fragments<C::FM>(sa, q, wm * C::WTM, kk, lane, fa[q]);
+      for (int q = 0; q < PA; ++q) LA::template fragments<C::FM>(now, q, wm * C::WTM, kk, lane, fa[q]);
       // small plane products first
 #pragma unroll
       for (int sum = (PA == 3 || PB == 3) ? 2 : 0; sum >= 0; --sum)
@@ -553,6 +524,15 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
               acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[qb][i], fa[qa][j], acc[i][j], 0, 0, 0);
         }
     }
+  };
+  if (s0 < s1) load(lds, s0);
+  for (int64_t s = s0; s < s1; ++s) {
+    const int buf = (int)(s - s0) & 1;
+    // this wave's loads of stage s are in LDS; after the barrier everyone's are, and nobody reads the
+    // other buffer any more
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    stage(lds + (buf ^ 1) * C::kStage, lds + buf * C::kStage, s);
   }
 
   // ------------------------------------------------------------------------------------------
