@@ -494,45 +494,101 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 #pragma unroll
     for (int j = 0; j < C::FM; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  // One stage: its fragments and their products, while the next stage comes in. The addresses are __restrict:
-  // without it the compiler takes every transposing read to depend on the loads into LDS in flight and waits
-  // for them first.
   auto load = [&](char* at, int64_t step) __attribute__((always_inline)) {
     la.load(at, step, p.k_half);
     lb.load(at + PA * TM * BK * 2, step, p.k_half);
   };
-  auto stage = [&](char* __restrict next, const char* __restrict now, int64_t s) __attribute__((always_inline)) {
-    if (s + 1 < s1) load(next, s + 1);
-#pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      bf16x8 fa[PA][C::FM], fb[PB][C::FN];
-#pragma unroll
-      for (int q = 0; q < PB; ++q) LB::template fragments<C::FN>(now + PA * TM * BK * 2, q, wn * C::WTN, kk, lane, fb[q]);
-#pragma unroll
-      for (int q = 0; q < PA; ++q) LA::template fragments<C::FM>(now, q, wm * C::WTM, kk, lane, fa[q]);
-      // small plane products first
-#pragma unroll
-      for (int sum = (PA == 3 || PB == 3) ? 2 : 0; sum >= 0; --sum)
-#pragma unroll
-        for (int qa = 0; qa < PA; ++qa) {
-          const int qb = sum - qa;
-          if (qb < 0 || qb >= PB) continue;
-#pragma unroll
-          for (int i = 0; i < C::FN; ++i)
-#pragma unroll
-            for (int j = 0; j < C::FM; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[qb][i], fa[qa][j], acc[i][j], 0, 0, 0);
-        }
-    }
+  struct Set {
+    bf16x8 a[PA][C::FM], b[PB][C::FN];
   };
-  if (s0 < s1) load(lds, s0);
-  for (int64_t s = s0; s < s1; ++s) {
-    const int buf = (int)(s - s0) & 1;
-    // this wave's loads of stage s are in LDS; after the barrier everyone's are, and nobody reads the
-    // other buffer any more
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  auto read = [&](const char* at, int kk, Set& t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < PB; ++q) LB::template fragments<C::FN>(at + PA * TM * BK * 2, q, wn * C::WTN, kk, lane, t.b[q]);
+#pragma unroll
+    for (int q = 0; q < PA; ++q) LA::template fragments<C::FM>(at, q, wm * C::WTM, kk, lane, t.a[q]);
+  };
+  auto multiply = [&](const Set& t) __attribute__((always_inline)) {
+    // small plane products first
+#pragma unroll
+    for (int sum = (PA == 3 || PB == 3) ? 2 : 0; sum >= 0; --sum)
+#pragma unroll
+      for (int qa = 0; qa < PA; ++qa) {
+        const int qb = sum - qa;
+        if (qb < 0 || qb >= PB) continue;
+#pragma unroll
+        for (int i = 0; i < C::FN; ++i)
+#pragma unroll
+          for (int j = 0; j < C::FM; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t.b[qb][i], t.a[qa][j], acc[i][j], 0, 0, 0);
+      }
+  };
+  constexpr int kVmcnt0 = 0x0f70;  // s_waitcnt vmcnt(0), the other counters as they are
+  // The stages' addresses are __restrict: without it the compiler takes every transposing read to depend on the
+  // loads into LDS in flight and waits for them first.
+  if constexpr (C::kThreads == 512) {
+    // Two groups of four waves, one of each on a SIMD, half a step apart: while one reads its fragments the other
+    // has the matrix cores. Every phase ends at a barrier; the second group starts one barrier late and the first
+    // ends with one more.
+    //   phase 2 i:      first reads set i          second multiplies set i - 1
+    //   phase 2 i + 1:  first multiplies set i     second reads set i
+    // A group loads its share of stage s + 1 as it begins to read stage s: by then both groups' reads of stage s - 1,
+    // whose place it takes, have ended (the other's last one a barrier ago). Both wait for their shares before
+    // the barrier in front of the first group's first read of stage s + 1.
+    // The barrier alone: __syncthreads would wait for the loads into LDS at every one.
+    constexpr int kLgkmcnt0 = 0xc07f;
+    auto phase = [&]() __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+    };
+    const bool second = wave >= 4;
+    auto stage = [&](char* __restrict next, const char* __restrict now, int64_t s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int kk = 0; kk < BK / 32; ++kk) {
+        Set f;
+        if (kk == 0 && s + 1 < s1) load(next, s + 1);
+        read(now, kk, f);
+        if (kk == BK / 32 - 1 && second) __builtin_amdgcn_s_waitcnt(kVmcnt0);
+        __builtin_amdgcn_s_waitcnt(kLgkmcnt0);
+        phase();
+        __builtin_amdgcn_s_setprio(1);
+        multiply(f);
+        __builtin_amdgcn_s_setprio(0);
+        if (kk == BK / 32 - 1 && !second) __builtin_amdgcn_s_waitcnt(kVmcnt0);
+        phase();
+      }
+    };
+    if (s0 < s1) load(lds, s0);
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
     __syncthreads();
-    stage(lds + (buf ^ 1) * C::kStage, lds + buf * C::kStage, s);
+    if (second) phase();
+    for (int64_t s = s0; s < s1; ++s) {
+      const int buf = (int)(s - s0) & 1;
+      stage(lds + (buf ^ 1) * C::kStage, lds + buf * C::kStage, s);
+    }
+    if (!second) phase();
+  } else {
+    // one stage: its fragments and their products, while the next stage comes in
+    auto stage = [&](char* __restrict next, const char* __restrict now, int64_t s) __attribute__((always_inline)) {
+      if (s + 1 < s1) load(next, s + 1);
+#pragma unroll
+      for (int kk = 0; kk < BK / 32; ++kk) {
+        Set f;
+        read(now, kk, f);
+        multiply(f);
+      }
+    };
+    if (s0 < s1) load(lds, s0);
+    for (int64_t s = s0; s < s1; ++s) {
+      const int buf = (int)(s - s0) & 1;
+      // this wave's loads of stage s are in LDS; after the barrier everyone's are, and nobody reads the
+      // other buffer any more
+      __builtin_amdgcn_s_waitcnt(kVmcnt0);
+      __syncthreads();
+      stage(lds + (buf ^ 1) * C::kStage, lds + buf * C::kStage, s);
+    }
   }
 
   // ------------------------------------------------------------------------------------------
