@@ -1436,8 +1436,8 @@ def embedding(index, table, scale=1.0, padding_idx=None):
     if index.device != table.device:
         raise _lib.AimxError("aimx.embedding: index and table on one device")
     V = table.shape[0]
-    if V >= 2 ** 31 - 1 or index.numel() >= 2 ** 31 - 1 or table.shape[1] > 1 << 24:
-        raise _lib.AimxError("aimx.embedding: at most 2^31 - 2 rows and indices, 2^24 columns")
+    if V >= 2 ** 31 - 1 or index.numel() >= 2 ** 31 - 1 or table.shape[1] > 1 << 21:
+        raise _lib.AimxError("aimx.embedding: at most 2^31 - 2 rows and indices, 2^21 columns")
     if padding_idx is not None and not -V <= padding_idx < V:
         raise _lib.AimxError(f"aimx.embedding: padding_idx in [-{V}, {V})")
     pad = -1 if padding_idx is None else int(padding_idx) % V

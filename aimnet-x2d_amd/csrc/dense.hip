@@ -396,7 +396,7 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     p.rows = t;
     p.rows_plane = plane;
     const Plan at = (px == 1 && k.planes == 1) ? plan_one(M, N * H, p.K, false) : plan_split(M, N * H, p.K, false);
-    parts = cdiv(M, at.tile_m) * at.waves_m;
+    parts = cdiv(M, at.rows) * kWavesM;
     if (has_db) sums = p.sums = ws.take<float>(parts * H * N);
     product(c, ws, p, px, k.planes, H == 2 ? kGatedGrad : kDenseGrad, kNone, k.fp32);
   } else {

@@ -11,18 +11,13 @@ using Small = Config<1, 1, 64, 64, 2, 2, 64>;     // 4 waves of 32 x 32, 32 KB: 
 
 }  // namespace
 
+// At 20480 x 512 (K = 4096) 160 large tiles take 119 us, in two k ranges 131 and 19 for their sum; at
+// 20480 x 2048 (K = 512) three rounds of large tiles take 80 us and five of middle ones 68.
 Plan plan_one(int64_t M, int64_t columns, int64_t K, bool may_split) {
-  auto tiles = [&](int64_t t, int64_t u) { return std::max<int64_t>(1, cdiv(M, t) * cdiv(columns, u)); };
-  const int64_t steps = K / 64;
-  const int64_t most = may_split ? std::max<int64_t>(1, steps / 8) : 1;  // a k range has 8 steps at least
+  static const Shape shapes[] = {{0, 256, 256, 64, 1, 1.74, 9.}, {1, 128, 128, 64, 2, 1.08, 4.5}, {2, 64, 64, 64, 5, 0.85, 3.}};
   const int64_t force = tune_i64("AIMX_DENSE_TILE", -1), fs = tune_i64("AIMX_DENSE_SPLITS", 0);
-  Plan r{2, 1, 2, 64};
-  if (tiles(256, 256) * most >= 192) r = {0, (int)std::min(most, cdiv(192, tiles(256, 256))), 2, 256};
-  else if (tiles(128, 128) * most >= 192) r = {1, (int)std::min(most, cdiv(384, tiles(128, 128))), 2, 128};
-  else r.splits = (int)std::min(most, cdiv(512, tiles(64, 64)));
-  if (force >= 0) r.tile = (int)force, r.tile_m = force == 0 ? 256 : force == 1 ? 128 : 64;
-  if (fs > 0) r.splits = (int)std::min(may_split ? fs : 1, steps);
-  return r;
+  if (force >= 0) return pick(shapes + force, 1, M, columns, K, may_split && fs != 1);
+  return pick(shapes, 3, M, columns, K, may_split && fs != 1);
 }
 
 int launch_one(const Problem& p, int tile, int epi, int across, bool fp32, hipStream_t st) {

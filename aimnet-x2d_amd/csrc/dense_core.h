@@ -90,6 +90,7 @@ enum Across : int { kNone = 0, kB = 1, kBoth = 2 };
 template <int PA_, int PB_, int TM_, int TN_, int WGM_, int WGN_, int BK_>
 struct Config {
   static constexpr int PA = PA_, PB = PB_, TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, BK = BK_;
+  static_assert(WGM == 2, "kWavesM");
   static constexpr int kThreads = WGM * WGN * kWave;
   static constexpr int WTM = TM / WGM, WTN = TN / WGN, FM = WTM / 16, FN = WTN / 16;
   static constexpr int U = BK / 8;                   // 16-byte units of a row
@@ -599,13 +600,41 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
 #endif
 }
 
-// A tile shape (0: the largest) and the number of k ranges of one launch.
+// A tile shape and the number of k ranges of one launch, picked by an estimate of its time.
+struct Shape {
+  int tile;        // index of the launchers
+  int64_t rows, cols, bk;
+  int per_cu;      // workgroups that fit a CU
+  double step, end;  // us: one k step of a workgroup with its CU full, its prologue and epilogue (measured)
+};
 struct Plan {
   int tile, splits;
-  int waves_m;  // rows of waves of the tile, over tile_m rows: the column sums' parts are per wave row
-  int64_t tile_m;
+  int64_t rows;
 };
+constexpr int kWavesM = 2;  // rows of waves of every tile: a tile leaves that many parts of column sums
+constexpr int kCus = 256;
 // `columns`: of both halves together. may_split: a plain product whose partial sums may go to slabs.
+inline Plan pick(const Shape* shapes, int n, int64_t M, int64_t columns, int64_t K, bool may_split) {
+  Plan best{shapes[0].tile, 1, shapes[0].rows};
+  double least = 1e30;
+  for (int i = 0; i < n; ++i) {
+    const Shape& s = shapes[i];
+    const int64_t tiles = std::max<int64_t>(1, cdiv(M, s.rows) * cdiv(columns, s.cols)), steps = K / s.bk;
+    const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(steps * s.bk / 256, 64)) : 1;
+    for (int64_t k = 1; k <= most; ++k) {
+      const int64_t all = tiles * k, slots = (int64_t)kCus * s.per_cu, rest = all % slots;
+      // workgroups that share a CU with fewer are faster, alone about twice as fast as among three
+      const double part = rest == 0 ? 0. : s.per_cu == 1 ? 1. : std::max(0.47, 0.2 + 0.8 * (double)rest / (double)slots);
+      const double rounds = (double)(all / slots) + part;
+      double t = rounds * ((double)cdiv(steps, k) * s.step + s.end);
+      // the slabs are written and read again, about 4.5 TB/s, by one more launch
+      if (k > 1) t += 5. + (double)(6 * k + 4) * (double)M * (double)columns / 4.5e6;
+      if (t < least) least = t, best = Plan{s.tile, (int)k, s.rows};
+      if (all > 16 * slots) break;
+    }
+  }
+  return best;
+}
 Plan plan_one(int64_t M, int64_t columns, int64_t K, bool may_split);
 Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split);
 // Launchers (dense_bf16.hip: one plane a side; dense_split.hip: three planes on one side or both, fp32 tensors).

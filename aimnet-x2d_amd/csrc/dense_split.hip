@@ -6,7 +6,9 @@ namespace dense {
 namespace {
 
 template <int PA, int PB>
-using Medium = Config<PA, PB, 128, 128, 2, 2, 32>;  // 4 waves of 64 x 64; 96 KB of LDS at 3 x 3 planes
+using Large = Config<PA, PB, 256, 128, 2, 4, 32>;  // 8 waves of 128 x 32; 144 KB of LDS at 3 x 3 planes
+template <int PA, int PB>
+using Medium = Config<PA, PB, 128, 128, 2, 4, 32>;  // 8 waves of 64 x 32; 96 KB of LDS at 3 x 3 planes
 template <int PA, int PB>
 using Small = Config<PA, PB, 64, 64, 2, 2, 32>;  // 4 waves of 32 x 32; 48 KB
 
@@ -38,14 +40,16 @@ int go(const Problem& p, int pa, int pb, int epi, int across, hipStream_t st) {
 
 }  // namespace
 
+// At 9186 rows, 256 -> 2 x 683: 3168 small tiles 67 us, 792 middle ones 72; at 20480 rows, 512 -> 2 x 2048: 745 and 595.
 Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split) {
-  auto tiles = [&](int64_t t) { return std::max<int64_t>(1, cdiv(M, t) * cdiv(columns, t)); };
-  const int64_t most = may_split ? std::max<int64_t>(1, K / 256) : 1;  // a k range has 8 steps at least
-  if (tiles(128) * most >= 192) return {0, (int)std::min(most, cdiv(256, tiles(128))), 2, 128};
-  return {1, (int)std::min(most, cdiv(512, tiles(64))), 2, 64};
+  static const Shape shapes[] = {{0, 128, 128, 32, 1, 1.1, 9.}, {1, 64, 64, 32, 3, 1.5, 4.}, {2, 256, 128, 32, 1, 1.95, 12.}};
+  const int64_t force = tune_i64("AIMX_DENSE_SPLIT_TILE", -1);
+  if (force >= 0) return pick(shapes + force, 1, M, columns, K, may_split);
+  return pick(shapes, 3, M, columns, K, may_split);
 }
 
 int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, hipStream_t st) {
+  if (tile == 2) return go<Large>(p, pa, pb, epi, across, st);
   return tile == 0 ? go<Medium>(p, pa, pb, epi, across, st) : go<Small>(p, pa, pb, epi, across, st);
 }
 

@@ -214,8 +214,9 @@ struct Runs {
   int64_t n, V, D, ldd, seg, segs;
   int64_t slices;  // column slices of a row
   int32_t group;   // lanes of a slice
-  float* head;     // [segs][D]: the part of a run that began before the segment
-  float* tail;     // [segs][D]: the part of a run that goes on behind it and began inside
+  int64_t ldp;     // D rounded up to 4
+  float* head;     // [segs][ldp]: the part of a run that began before the segment
+  float* tail;     // [segs][ldp]: the part of a run that goes on behind it and began inside
   float scale;
 };
 
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(256) void k_token_runs(const Runs a, const T* __res
         if (ends || last) {
           if (key[j] != none) {
             if (from_before || !ends) {
-              float* part = (from_before ? a.head : a.tail) + seg * a.D + c;
+              float* part = (from_before ? a.head : a.tail) + seg * a.ldp + c;
 #pragma unroll
               for (int e = 0; e < VEC; ++e) part[e] = acc[e];
             } else {
@@ -275,45 +276,83 @@ __global__ __launch_bounds__(256) void k_token_runs(const Runs a, const T* __res
   }
 }
 
-// A workgroup per segment whose last run goes on: 4 waves add the run's partial rows, a quarter each, in order
+// The runs that cross segments, 64 columns a workgroup: each of its 16 groups of 16 lanes takes a segment whose last run
+// goes on and began in it, and adds the partial rows in order; runs over 16 segments and more are left for the
+// whole workgroup, a contiguous part for each group and the groups' sums in order. (A workgroup per segment spent
+// 25 us at 65536 tokens finding that most have nothing to do.)
 template <typename T>
 __global__ __launch_bounds__(256) void k_token_join(const Runs a, T* __restrict__ dtable) {
-  __shared__ float part[4][64];
-  const int64_t seg = blockIdx.x, p1 = (seg + 1) * a.seg;
-  if (p1 >= a.n) return;
-  const uint32_t key = a.key[p1];
-  if (key == (uint32_t)a.V || a.key[p1 - 1] != key) return;
-  if (seg > 0 && a.key[seg * a.seg - 1] == key) return;  // it began further in front
-  int64_t lo = p1, hi = a.n;  // the run's end
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (a.key[mid] == key) lo = mid + 1;
-    else hi = mid;
+  __shared__ float part[16][64];
+  __shared__ int32_t behind, longs[16];
+  const int lane = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t c = blockIdx.y * (int64_t)64 + lane * 4;
+  auto at = [&](const float* p, int64_t seg) { return *reinterpret_cast<const floatx4*>(p + seg * a.ldp + c); };
+  {
+    const int64_t seg = blockIdx.x * (int64_t)16 + g, p1 = (seg + 1) * a.seg;
+    bool owner = p1 < a.n;
+    uint32_t key = 0;
+    if (owner) {
+      key = a.key[p1];
+      owner = key != (uint32_t)a.V && a.key[p1 - 1] == key && (seg == 0 || a.key[seg * a.seg - 1] != key);
+    }
+    // the segments behind that begin with the run, 16 looked at
+    const int64_t t = seg + 1 + lane;
+    const bool same = owner && t < a.segs && a.key[t * a.seg] == key;
+    const uint32_t mask = (uint32_t)(__ballot(same) >> (threadIdx.x & 48)) & 0xffffu;
+    const int parts = __ffs((int)(~mask)) - 1;  // bit 16 of ~mask is set: at most 16
+    if (lane == 0) longs[g] = owner && parts == 16;
+    if (owner && parts < 16 && c < a.ldp) {
+      floatx4 s = at(a.tail, seg);
+      for (int j = 0; j < parts; ++j) s += at(a.head, seg + 1 + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.D) {
+          Cols<T, 1> o;
+          o.v[0] = s[e];
+          o.store(dtable + (int64_t)key * a.D + c + e, a.scale);
+        }
+    }
   }
-  const int64_t parts = (lo - 1) / a.seg - seg;  // heads of the segments behind
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t t0 = seg + 1 + parts * w / 4, t1 = seg + 1 + parts * (w + 1) / 4;
-  for (int64_t c0 = 0; c0 < a.D; c0 += 64) {
-    const int64_t c = c0 + lane;
-    float s = 0.f;
-    if (c < a.D) {
-      if (w == 0) s = a.tail[seg * a.D + c];
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) {
+    if (!longs[k]) continue;
+    const int64_t seg = blockIdx.x * (int64_t)16 + k;
+    const uint32_t key = a.key[(seg + 1) * a.seg];
+    int64_t parts = 0;
+    for (int64_t t0 = seg + 1;; t0 += 256) {
+      if (threadIdx.x == 0) behind = 256;
+      __syncthreads();
+      const int64_t t = t0 + threadIdx.x;
+      if (t >= a.segs || a.key[t * a.seg] != key) atomicMin(&behind, (int32_t)threadIdx.x);
+      __syncthreads();
+      const int32_t got = behind;
+      parts += got;
+      __syncthreads();
+      if (got < 256) break;
+    }
+    const int64_t t0 = seg + 1 + parts * g / 16, t1 = seg + 1 + parts * (g + 1) / 16;
+    floatx4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.ldp) {
+      if (g == 0) s = at(a.tail, seg);
       int64_t t = t0;
       for (; t + 8 <= t1; t += 8) {
-        float v[8];
+        floatx4 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = a.head[(t + j) * a.D + c];
+        for (int j = 0; j < 8; ++j) v[j] = at(a.head, t + j);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += v[j];
       }
-      for (; t < t1; ++t) s += a.head[t * a.D + c];
+      for (; t < t1; ++t) s += at(a.head, t);
     }
-    part[w][lane] = s;
+    *reinterpret_cast<floatx4*>(&part[g][lane * 4]) = s;
     __syncthreads();
-    if (w == 0 && c < a.D) {
+    const int64_t col = blockIdx.y * (int64_t)64 + threadIdx.x;
+    if (threadIdx.x < 64 && col < a.D) {
       Cols<T, 1> o;
-      o.v[0] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-      o.store(dtable + (int64_t)key * a.D + c, a.scale);
+      o.v[0] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o.v[0] += part[i][threadIdx.x];
+      o.store(dtable + (int64_t)key * a.D + col, a.scale);
     }
     __syncthreads();
   }
@@ -322,7 +361,7 @@ __global__ __launch_bounds__(256) void k_token_join(const Runs a, T* __restrict_
 // --------------------------------------------------------------------------------------------
 inline bool args_ok(int32_t dtype, int64_t n, int64_t V, int64_t D) {
   return (dtype == AIMX_DTYPE_F32 || dtype == AIMX_DTYPE_BF16) && n >= 0 && n < INT32_MAX && V >= 1 && V < INT32_MAX &&
-         D >= 1 && D <= (int64_t)1 << 24;
+         D >= 1 && D <= (int64_t)1 << 21;  // 64 columns a workgroup in the grid's y
 }
 
 struct Layout {
@@ -339,7 +378,7 @@ Layout layout(char* base, int64_t n, int64_t V, int64_t D) {
     used += (b + 255) & ~(size_t)255;
     return p;
   };
-  // at least 4 rounds of 64 items for a wave, at most kMaxChunks waves
+  // 4 rounds of 64 items for a wave at least (65536 tokens, a pass: 14.6 us; 1 round: 16.4), at most kMaxChunks waves
   l.s.chunk = std::max<int64_t>(256, cdiv(cdiv(n, kMaxChunks), 64) * 64);
   l.s.chunks = cdiv(n, l.s.chunk);
   // rows of a segment: enough segments to fill the card, few enough that joining a frequent token's is short
@@ -351,8 +390,9 @@ Layout layout(char* base, int64_t n, int64_t V, int64_t D) {
     l.s.id[i] = (uint32_t*)take((size_t)n * 4);
   }
   l.s.hist = (int32_t*)take((size_t)l.s.chunks * 256 * 4);
-  l.r.head = (float*)take((size_t)l.r.segs * D * 4);
-  l.r.tail = (float*)take((size_t)l.r.segs * D * 4);
+  l.r.ldp = (D + 3) / 4 * 4;
+  l.r.head = (float*)take((size_t)l.r.segs * l.r.ldp * 4);
+  l.r.tail = (float*)take((size_t)l.r.segs * l.r.ldp * 4);
   l.bytes = used;
   return l;
 }
@@ -417,7 +457,8 @@ int grad(const int64_t* index, int64_t n, const T* dy, int64_t ldd, int64_t V, i
   else hipLaunchKernelGGL((k_token_runs<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, r, dy, dtable);
   AIMX_CHECK_LAUNCH();
   if (r.segs > 1) {
-    hipLaunchKernelGGL((k_token_join<T>), dim3((unsigned)(r.segs - 1)), dim3(256), 0, st, r, dtable);
+    hipLaunchKernelGGL((k_token_join<T>), dim3((unsigned)cdiv(r.segs - 1, 16), (unsigned)cdiv(D, 64)), dim3(256), 0, st, r,
+                       dtable);
     AIMX_CHECK_LAUNCH();
   }
   return AIMX_OK;

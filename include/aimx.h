@@ -649,7 +649,7 @@ int aimx_unpack8(int32_t dtype, const int8_t* q, const int8_t* exps, int64_t M, 
  *   backward  dtable[v] = scale * sum over i with index[i] = v of dy[i], ascending i, in fp32 (deterministic:
  *             tokens sorted by id, runs summed in order); every row of dtable [V, D] is written (16-byte aligned)
  * An index outside [0, V) gives a zero row and no gradient; rows equal to padding_idx (-1: none) give no
- * gradient. n, V < 2^31 - 1.
+ * gradient. n, V < 2^31 - 1, D <= 2^21.
  * ------------------------------------------------------------------------------------------ */
 int aimx_token_embedding_forward(int32_t dtype, const int64_t* index, int64_t n, const void* table, int64_t V,
                                  int64_t D, float scale, void* out, aimx_stream_t stream);
