@@ -1147,27 +1147,18 @@ _DTYPES = {_F32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 PACK8_GROUP = 32
 
 
-class _on:
-    """Makes `device` the current one for the kernels launched inside, if it is not already."""
-
-    def __init__(self, device):
-        self.device, self.back = device, None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if self.device.index is not None and self.device.index != now:
-            self.back = now
-            torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
-        return False
+def _launch(device, what, fn, *args):
+    """fn(*args, stream): a C call that enqueues on `device`'s current stream, with `device` current."""
+    now = torch.cuda.current_device()
+    if device.index == now:
+        return check(fn(*args, stream_ptr(device)), what)
+    with torch.cuda.device(device):
+        return check(fn(*args, stream_ptr(device)), what)
 
 
 def _matrix(what, name, t):
     """(t as [M, K] rows, row stride); t has unit column stride or is copied."""
-    t, ld = _rows(t.reshape(-1, t.shape[-1]))
+    t, ld = _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
     if ld > 1 << 21:
         raise _lib.AimxError(f"aimx.{what}: {name} has a row stride over 2^21 elements")
     return t, ld
@@ -1192,14 +1183,12 @@ def _pack8(what, x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise _lib.AimxError(f"aimx.{what}: the last dimension must hold at least one value")
     _lib.require_device(x)
-    x2, ld = _rows(x.reshape(-1, x.shape[-1]))
+    x2, ld = _rows(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     M, K = x2.shape
     kq = -(-K // PACK8_GROUP) * PACK8_GROUP
     q = torch.empty(M, kq, dtype=torch.int8, device=x.device)
     exps = torch.empty(M, kq // PACK8_GROUP, dtype=torch.int8, device=x.device)
-    with _on(x.device):
-        check(_lib.load().aimx_pack8(_DTYPES[x.dtype], ptr(x2), ld, M, K, ptr(q), ptr(exps), stream_ptr(x.device)),
-              "pack8")
+    _launch(x.device, "pack8", _lib.load().aimx_pack8, _DTYPES[x.dtype], ptr(x2), ld, M, K, ptr(q), ptr(exps))
     return Packed8(q, exps, tuple(x.shape), x.dtype)
 
 
@@ -1218,9 +1207,8 @@ def unpack8(packed, dtype=None):
         raise _lib.AimxError(f"aimx.unpack8: fp32 or bf16, got {dtype}")
     dev, K = packed.q.device, packed.shape[-1]
     out = torch.empty(packed.shape, dtype=dtype, device=dev)
-    with _on(dev):
-        check(_lib.load().aimx_unpack8(_DTYPES[dtype], ptr(packed.q), ptr(packed.exps), packed.q.shape[0], K, ptr(out),
-                                       K, stream_ptr(dev)), "unpack8")
+    _launch(dev, "unpack8", _lib.load().aimx_unpack8, _DTYPES[dtype], ptr(packed.q), ptr(packed.exps),
+            packed.q.shape[0], K, ptr(out), K)
     return out
 
 
@@ -1257,11 +1245,12 @@ def _dense_forward(x, ws, bs, res, act, prec, keep_pre):
     if keep_pre:
         pre = torch.empty(d.M, len(ws), -(-n // 8) * 8, dtype=_F32, device=dev)
         d.pre = ptr(pre)
-    with _on(dev):
-        d.workspace_bytes = lib.aimx_dense_workspace_bytes(ctypes.byref(d))
-        work = _workspace(d.workspace_bytes, dev)
-        d.workspace = ptr(work)
-        check(lib.aimx_dense_forward(ctypes.byref(d), stream_ptr(dev)), "dense_forward")
+    arg = ctypes.byref(d)
+    nbytes = lib.aimx_dense_workspace_bytes(arg)
+    if nbytes:
+        work = _workspace(nbytes, dev)
+        d.workspace, d.workspace_bytes = ptr(work), nbytes
+    _launch(dev, "dense_forward", lib.aimx_dense_forward, arg)
     return y, pre, x2
 
 
@@ -1319,11 +1308,11 @@ class _DenseFn(torch.autograd.Function):
             for i, t in enumerate(db):
                 g.db[i] = ptr(t)
         if dx is not None or dw is not None or db is not None:
-            with _on(dev):
-                g.workspace_bytes = lib.aimx_dense_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(g))
-                work = _workspace(g.workspace_bytes, dev)
-                g.workspace = ptr(work)
-                check(lib.aimx_dense_backward(ctypes.byref(d), ctypes.byref(g), stream_ptr(dev)), "dense_backward")
+            args = ctypes.byref(d), ctypes.byref(g)
+            g.workspace_bytes = lib.aimx_dense_backward_workspace_bytes(*args)
+            work = _workspace(g.workspace_bytes, dev)
+            g.workspace = ptr(work)
+            _launch(dev, "dense_backward", lib.aimx_dense_backward, *args)
         at = lambda v, i: v[i] if v is not None and i < len(v) and need[i + (1 if v is dw else 3)] else None  # noqa: E731
         return dx, at(dw, 0), at(dw, 1), at(db, 0), at(db, 1), dy if need[5] else None, None, None
 
@@ -1341,8 +1330,9 @@ def _dense_checks(what, x, ws, bs, act, res=None):
     if res is not None and res.shape != (*x.shape[:-1], n):
         raise _lib.AimxError(f"aimx.{what}: the residual has the result's shape {(*x.shape[:-1], n)}, got "
                              f"{tuple(res.shape)}")
+    dtype, device = x.dtype, x.device
     for t in (*ws, *bs, res):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+        if t is not None and (t.dtype != dtype or t.device != device):
             raise _lib.AimxError(f"aimx.{what}: every tensor has x's dtype and device ({x.dtype}, {x.device})")
     if max(ws[0].shape) > 1 << 21:
         raise _lib.AimxError(f"aimx.{what}: widths up to 2^21")
@@ -1353,7 +1343,11 @@ def _dense_checks(what, x, ws, bs, act, res=None):
 
 
 def _dense_apply(what, x, ws, bs, res, act, checkpoint8):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *ws, *bs, res)):
+    grad = False
+    if torch.is_grad_enabled():
+        for t in (x, *ws, *bs, res):
+            grad = grad or (t is not None and t.requires_grad)
+    if grad:
         if x.numel() // x.shape[-1] > 1 << 22:
             raise _lib.AimxError(f"aimx.{what}: at most 2^22 rows where gradients are asked for")
         two = len(ws) == 2
@@ -1392,10 +1386,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", checkpoint
 def _embedding_forward(index, table, scale):
     D = table.shape[1]
     out = torch.empty(*index.shape, D, dtype=table.dtype, device=table.device)
-    with _on(table.device):
-        check(_lib.load().aimx_token_embedding_forward(_DTYPES[table.dtype], ptr(index), index.numel(), ptr(table),
-                                                       table.shape[0], D, scale, ptr(out), stream_ptr(table.device)),
-              "token_embedding_forward")
+    _launch(table.device, "token_embedding_forward", _lib.load().aimx_token_embedding_forward, _DTYPES[table.dtype],
+            ptr(index), index.numel(), ptr(table), table.shape[0], D, scale, ptr(out))
     return out
 
 
@@ -1414,14 +1406,13 @@ class _Embedding(torch.autograd.Function):
         index, = ctx.saved_tensors
         (V, D), dtype = ctx.table
         dev = dy.device
-        dy2, ldd = _rows(dy.reshape(-1, D))
+        dy2, ldd = _rows(dy if dy.dim() == 2 else dy.reshape(-1, D))
         grad = torch.empty(V, D, dtype=dtype, device=dev)
-        with _on(dev):
-            nbytes = lib.aimx_token_embedding_backward_workspace_bytes(_DTYPES[dtype], index.numel(), V, D)
-            work = _workspace(nbytes, dev)
-            check(lib.aimx_token_embedding_backward(_DTYPES[dtype], ptr(index), index.numel(), ptr(dy2), ldd, V, D,
-                                                    ctx.scale, ctx.padding_idx, ptr(grad), ptr(work), nbytes,
-                                                    stream_ptr(dev)), "token_embedding_backward")
+        n, kind = index.numel(), _DTYPES[dtype]
+        nbytes = lib.aimx_token_embedding_backward_workspace_bytes(kind, n, V, D)
+        work = _workspace(nbytes, dev)
+        _launch(dev, "token_embedding_backward", lib.aimx_token_embedding_backward, kind, ptr(index), n, ptr(dy2), ldd,
+                V, D, ctx.scale, ctx.padding_idx, ptr(grad), ptr(work), nbytes)
         return None, grad, None, None
 
 
@@ -1442,7 +1433,7 @@ def embedding(index, table, scale=1.0, padding_idx=None):
         raise _lib.AimxError(f"aimx.embedding: padding_idx in [-{V}, {V})")
     pad = -1 if padding_idx is None else int(padding_idx) % V
     _lib.require_device(table)
-    index = index.to(torch.int64).contiguous()
+    index = (index if index.dtype == torch.int64 else index.long()).contiguous()
     if torch.is_grad_enabled() and table.requires_grad:
         return _Embedding.apply(index, table, float(scale), pad)
     return _embedding_forward(index, table.contiguous(), float(scale))
