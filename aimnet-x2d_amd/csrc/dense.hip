@@ -35,7 +35,6 @@ struct Segment {
   uint16_t* dst;
   int64_t ldd, plane;
   int64_t first;  // first work item of this segment
-  int32_t vec;    // 16-byte loads (kQ8: 8-byte ones, always)
 };
 struct Segments {
   Segment s[3];
@@ -43,27 +42,7 @@ struct Segments {
   int64_t items;
 };
 
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef int8_t i8x8 __attribute__((ext_vector_type(8)));
-
-// 8 values from p, `left` of which exist (the others: zero)
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int64_t left, float (&v)[8]) {
-  if (vec && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-    } else {
-      const u16x8 a = *reinterpret_cast<const u16x8*>(p);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = from_bf16(a[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? load1(p + i) : 0.f;
-  }
-}
 
 template <int PL>
 __device__ __forceinline__ void store_planes8(uint16_t* dst, int64_t plane, const float (&v)[8]) {
@@ -100,9 +79,9 @@ __global__ __launch_bounds__(256) void k_stage(const Segments a) {
       for (int j = 0; j < 8; ++j)
         v[j] = c + j < s.C ? (e == 127 ? __uint_as_float(0x7fc00000u) : ldexpf((float)q[j], e)) : 0.f;
     } else if constexpr (SRC == kF32) {
-      load8((const float*)s.src + r * s.ld + c, s.vec, s.C - c, v);
+      load8((const float*)s.src + r * s.ld + c, s.C - c, v);
     } else {
-      load8((const uint16_t*)s.src + r * s.ld + c, s.vec, s.C - c, v);
+      load8((const uint16_t*)s.src + r * s.ld + c, s.C - c, v);
     }
     store_planes8<PL>(s.dst + r * s.ldd + c, s.plane, v);
   }
@@ -117,7 +96,7 @@ struct Dpre {
   uint16_t* rows;
   int64_t plane;
   float* sums;  // [cdiv(M, 128)][halves * N]
-  int32_t act, vec;
+  int32_t act;
 };
 constexpr int kDpreRows = 128;
 template <typename T, int PL, int HALVES>
@@ -132,10 +111,10 @@ __global__ __launch_bounds__(256) void k_dpre(const Dpre a) {
     const int64_t m = tm * kDpreRows + j * 32 + r;
     if (m >= a.M) continue;
     float d[8], g[8], u[8], o[8];
-    load8((const T*)a.dy + m * a.ldd + n, a.vec, a.N - n, d);
+    load8((const T*)a.dy + m * a.ldd + n, a.N - n, d);
     if (a.pre && n < a.N8) {
-      load8(a.pre + m * HALVES * a.N8 + n, true, 8, g);
-      if constexpr (HALVES == 2) load8(a.pre + m * HALVES * a.N8 + a.N8 + n, true, 8, u);
+      load8(a.pre + m * HALVES * a.N8 + n, 8, g);
+      if constexpr (HALVES == 2) load8(a.pre + m * HALVES * a.N8 + a.N8 + n, 8, u);
     }
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) {
@@ -194,18 +173,17 @@ __global__ __launch_bounds__(256) void k_reduce_slabs(const Problem p) {
   const int64_t w = (p.N + 3) / 4, items = p.M * w;
   for (int64_t it = blockIdx.x * (int64_t)256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
     const int64_t m = it / w, n = (it - m * w) * 4, left = p.N - n;
-    const bool v4 = p.vec && left >= 4;
     floatx4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) v += load4(p.slab + ((int64_t)s * p.M + m) * p.N + n, v4, left);
-    if (p.bias) v += load4((const T*)p.bias + n, v4, left);
+    for (int s = 0; s < p.splits; ++s) v += load4(p.slab + ((int64_t)s * p.M + m) * p.N + n, left);
+    if (p.bias) v += load4((const T*)p.bias + n, left);
     if (p.pre) *reinterpret_cast<floatx4*>(p.pre + m * p.n8 + n) = v;
     if (p.act >= 0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = act_fwd(p.act, v[e]);
     }
-    if (p.res) v += load4((const T*)p.res + m * p.ldr + n, v4, left);
+    if (p.res) v += load4((const T*)p.res + m * p.ldr + n, left);
     const int64_t r = m < p.y_rows ? m : m - p.y_rows;
-    if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, v, v4, left);
+    if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, v, left);
   }
 }
 
@@ -246,7 +224,6 @@ void stage(Ctx& c, Segments& a, int src, int planes) {
   for (int i = 0; i < a.n; ++i) {
     a.s[i].first = a.items;
     a.items += a.s[i].R * (a.s[i].ldd / 8);
-    a.s[i].vec = aligned16(a.s[i].src) && a.s[i].ld % (src == kF32 ? 4 : 8) == 0;
   }
   if (a.items == 0) return;
   if (src == kF32) return planes == 3 ? stage_go<kF32, 3>(c, a) : stage_go<kF32, 1>(c, a);
@@ -263,11 +240,6 @@ void product(Ctx& c, Carve& ws, Problem p, int pa, int pb, int epi, int across, 
   p.splits = t.splits;
   if (t.splits > 1) p.slab = ws.take<float>((int64_t)t.splits * p.M * p.N);
   if (c.dry || c.rc) return;
-  // 8- and 16-byte accesses of 4 columns: every row of every tensor starts at a multiple of 4 elements
-  const size_t b = fp32 ? 4 : 2;
-  auto four = [&](const void* q, int64_t ld) { return !q || (((uintptr_t)q % (4 * b)) == 0 && ld % 4 == 0); };
-  p.vec = p.N % 4 == 0 && four(p.y, p.ldy) && four(p.y2, p.ldy) && four(p.res, p.ldr) && four(p.bias, 0) &&
-          four(p.bias2, 0);
   p.n8 = (p.N + 7) / 8 * 8;
   p.np = up64(p.N);
   if (p.k_half == 0) p.k_half = p.K;
@@ -309,7 +281,7 @@ bool in_place(const Kind& k, const void* p, int64_t ld, int64_t cols, bool along
 }
 
 void add(Segments& a, const void* src, const int8_t* exp, int64_t ld, int64_t R, int64_t C, uint16_t* dst, int64_t ldd) {
-  a.s[a.n++] = Segment{src, exp, ld, R, C, dst, ldd, R * ldd, 0, 0};
+  a.s[a.n++] = Segment{src, exp, ld, R, C, dst, ldd, R * ldd, 0};
 }
 
 // x (or its 8-bit form) as an operand; `along` if some product reads it along its rows
@@ -409,7 +381,6 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     a.N8 = (N + 7) / 8 * 8;
     a.pre = d->act >= 0 ? d->pre : nullptr;
     a.act = d->act;
-    a.vec = aligned16(g->dy) && g->ldd % (k.fp32 ? 4 : 8) == 0;
     if (d->act < 0 && in_place(k, g->dy, g->ldd, N, has_dx)) {
       rows = {(const uint16_t*)g->dy, nullptr, g->ldd, 0, M, N};
     } else if (has_dx || has_dw) {

@@ -28,6 +28,12 @@ namespace dense {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+// the same in memory at any element: gfx950 takes 8- and 16-byte accesses at such addresses (within 8 % of the aligned
+// rate), so no row needs an alignment
+typedef float floatx4e __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4e __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint16_t u16x8e __attribute__((ext_vector_type(8), aligned(2)));
 
 // fp32 -> bf16 bits, round to nearest even; NaN stays NaN
 __device__ __forceinline__ uint16_t to_bf16(float v) {
@@ -78,7 +84,7 @@ struct Problem {
   int64_t rows_plane;
   float* sums;           // backward epilogues, nullable: column sums [tiles of rows * WGM][halves * N]
   int64_t n8, np;        // N rounded up to 8, to 64
-  int32_t act, splits, vec;
+  int32_t act, splits;
 };
 
 // kDenseGrad / kGatedGrad: the product is the forward's, computed again; what leaves the kernel is the gradient
@@ -155,15 +161,15 @@ __device__ __forceinline__ float load1<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float load1<uint16_t>(const uint16_t* p) { return from_bf16(*p); }
 
-// four consecutive values; vec: the address is a multiple of 4 elements and all four exist
+// four consecutive values, `left` of which exist (the others: zero)
 template <typename T>
-__device__ __forceinline__ floatx4 load4(const T* p, bool vec, int64_t left) {
+__device__ __forceinline__ floatx4 load4(const T* p, int64_t left) {
   floatx4 v;
-  if (vec) {
+  if (left >= 4) {
     if constexpr (sizeof(T) == 4) {
-      v = *reinterpret_cast<const floatx4*>(p);
+      v = *reinterpret_cast<const floatx4e*>(p);
     } else {
-      const u16x4 h = *reinterpret_cast<const u16x4*>(p);
+      const u16x4 h = *reinterpret_cast<const u16x4e*>(p);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = from_bf16(h[i]);
     }
@@ -173,38 +179,16 @@ __device__ __forceinline__ floatx4 load4(const T* p, bool vec, int64_t left) {
   }
   return v;
 }
-// the same as loaded, converted where it is used
 template <typename T>
-struct Raw4 {
-  floatx4 f;
-  __device__ __forceinline__ void load(const T* p, bool vec, int64_t left) { f = load4(p, vec, left); }
-  __device__ __forceinline__ floatx4 get() const { return f; }
-};
-template <>
-struct Raw4<uint16_t> {
-  u16x4 h;
-  __device__ __forceinline__ void load(const uint16_t* p, bool vec, int64_t left) {
-    if (vec) {
-      h = *reinterpret_cast<const u16x4*>(p);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = i < left ? p[i] : (uint16_t)0;
-    }
-  }
-  __device__ __forceinline__ floatx4 get() const {
-    return floatx4{from_bf16(h[0]), from_bf16(h[1]), from_bf16(h[2]), from_bf16(h[3])};
-  }
-};
-template <typename T>
-__device__ __forceinline__ void store4(T* p, floatx4 v, bool vec, int64_t left) {
-  if (vec) {
+__device__ __forceinline__ void store4(T* p, floatx4 v, int64_t left) {
+  if (left >= 4) {
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<floatx4*>(p) = v;
+      *reinterpret_cast<floatx4e*>(p) = v;
     } else {
       u16x4 h;
 #pragma unroll
       for (int i = 0; i < 4; ++i) h[i] = to_bf16(v[i]);
-      *reinterpret_cast<u16x4*>(p) = h;
+      *reinterpret_cast<u16x4e*>(p) = h;
     }
   } else {
 #pragma unroll
@@ -215,6 +199,70 @@ __device__ __forceinline__ void store4(T* p, floatx4 v, bool vec, int64_t left) 
       }
   }
 }
+// 8 values from p, `left` of which exist (the others: zero)
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
+  if (left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const floatx4 a = *reinterpret_cast<const floatx4e*>(p), b = *reinterpret_cast<const floatx4e*>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+      const u16x8 a = *reinterpret_cast<const u16x8e*>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from_bf16(a[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? load1(p + i) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t left, const float (&v)[8]) {
+  if (left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<floatx4e*>(p) = floatx4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<floatx4e*>(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
+    } else {
+      u16x8 o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = to_bf16(v[i]);
+      *reinterpret_cast<u16x8e*>(p) = o;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) {
+        if constexpr (sizeof(T) == 4) p[i] = v[i];
+        else p[i] = to_bf16(v[i]);
+      }
+  }
+}
+
+// Four values loaded from up to 3 columns in front of where they belong (the last ones of a row whose length is no
+// multiple of 4), converted and shifted into place where they are used.
+template <typename T>
+struct Raw4 {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  typedef T t4e __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  t4 h;
+  __device__ __forceinline__ void load(const T* p) { h = *reinterpret_cast<const t4e*>(p); }
+  __device__ __forceinline__ floatx4 get() const {
+    if constexpr (sizeof(T) == 4) return h;
+    else return floatx4{from_bf16(h[0]), from_bf16(h[1]), from_bf16(h[2]), from_bf16(h[3])};
+  }
+  __device__ __forceinline__ floatx4 get(int shift) const {
+    const floatx4 v = get();
+    floatx4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = 0.f;
+#pragma unroll
+      for (int k = 0; e + k < 4; ++k) o[e] = shift == k ? v[e + k] : o[e];
+    }
+    return o;
+  }
+};
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -322,7 +370,7 @@ struct Loader {
   }
 };
 
-template <typename C, int EPI, typename T, bool VEC>
+template <typename C, int EPI, typename T, bool WIDE>
 __device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN][C::FM], int tm, int64_t m0, int64_t n0,
                                          int wm, int wn, int lane, int split) {
   constexpr int kHalves = EPI == kGated || EPI == kGatedGrad ? 2 : 1, FH = C::FN / kHalves;
@@ -334,28 +382,36 @@ __device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN]
 #pragma unroll
   for (int i = 0; i < FH; ++i) {
     nn[i] = n0 + wn * (C::WTN / kHalves) + i * 16 + fc * 4;
-    nl[i] = VEC ? min(nn[i], p.N - 4) : nn[i];
+    nl[i] = min(nn[i], p.N - 4);
     b0[i] = b1[i] = floatx4{0.f, 0.f, 0.f, 0.f};
     if constexpr (EPI != kSlab) {
-      if (p.bias) b0[i] = load4((const T*)p.bias + nl[i], VEC, p.N - nn[i]);
-      if (kHalves == 2 && p.bias2) b1[i] = load4((const T*)p.bias2 + nl[i], VEC, p.N - nn[i]);
+      if (p.bias) b0[i] = load4((const T*)p.bias + nn[i], p.N - nn[i]);
+      if (kHalves == 2 && p.bias2) b1[i] = load4((const T*)p.bias2 + nn[i], p.N - nn[i]);
     }
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) total[h][i] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   constexpr bool kRes = EPI == kPlain || kGrad;
+  const bool whole = p.N % 4 == 0;
+  // a row's operand: in flight where rows hold at least 4 columns, else read where it is used
+  auto operand = [&](const Raw4<T>& d, int64_t m, int i) __attribute__((always_inline)) -> floatx4 {
+    if constexpr (!WIDE) return load4((const T*)p.res + m * p.ldr + nn[i], p.N - nn[i]);
+    const int64_t shift = nn[i] - nl[i];
+    if (whole) return shift > 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : d.get();
+    return d.get((int)min(shift, (int64_t)4));
+  };
   // rows whose operands are in flight together, 16 registers of them
   constexpr int kMost = 16 / sizeof(T) / FH, kAhead = kMost < 1 ? 1 : kMost < C::FM ? kMost : C::FM;
 #pragma unroll
   for (int j0 = 0; j0 < C::FM; j0 += kAhead) {
     Raw4<T> d[kAhead][FH];
-    if constexpr (kRes) {
+    if constexpr (kRes && WIDE) {
       if (p.res) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           const int64_t m = min(m0 + wm * C::WTM + (j0 + j) * 16 + fr, p.M - 1);
 #pragma unroll
-          for (int i = 0; i < FH; ++i) d[j][i].load((const T*)p.res + m * p.ldr + nl[i], VEC, p.N - nn[i]);
+          for (int i = 0; i < FH; ++i) d[j][i].load((const T*)p.res + m * p.ldr + nl[i]);
         }
       }
     }
@@ -392,7 +448,7 @@ __device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN]
         floatx4 o = {a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
         if constexpr (kGrad) {
           floatx4 out[kHalves];
-          const floatx4 dd = VEC && left <= 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : d[jj][i].get();
+          const floatx4 dd = operand(d[jj][i], m, i);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if constexpr (kHalves == 2) {
@@ -422,13 +478,13 @@ __device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN]
             for (int q = 0; q < PL; ++q) *reinterpret_cast<u16x4*>(at + q * p.rows_plane) = w[q];
           }
         } else if constexpr (EPI == kSlab) {
-          store4(p.slab + ((int64_t)split * p.M + m) * p.N + n, o, VEC, left);
+          store4(p.slab + ((int64_t)split * p.M + m) * p.N + n, o, left);
         } else if constexpr (EPI == kGated) {
-          store4((T*)p.y + m * p.ldy + n, o * (acc[i + FH][j] + b1[i]), VEC, left);
+          store4((T*)p.y + m * p.ldy + n, o * (acc[i + FH][j] + b1[i]), left);
         } else {
-          if (p.res) o += d[jj][i].get();
+          if (p.res) o += operand(d[jj][i], m, i);
           const int64_t r = m < p.y_rows ? m : m - p.y_rows;
-          if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, o, VEC, left);
+          if (r < p.y_valid) store4((T*)(m < p.y_rows ? p.y : p.y2) + r * p.ldy + n, o, left);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -593,9 +649,9 @@ __global__ __launch_bounds__(C::kThreads) void k_dense(const Problem p, const in
   }
 
   // ------------------------------------------------------------------------------------------
-  // Where every row starts at a multiple of four elements, the epilogue's operands come by unconditional loads
-  // (of the last row and columns in place of those past the end), all in flight together.
-  if (p.vec) epilogue<C, EPI, T, true>(p, acc, tm, m0, n0, wm, wn, lane, split);
+  // The epilogue's operands come by unconditional loads (of the last row and the last four columns in place of those
+  // past the end), several rows' in flight together; rows of fewer than four columns have a form of their own.
+  if (p.N >= 4) epilogue<C, EPI, T, true>(p, acc, tm, m0, n0, wm, wn, lane, split);
   else epilogue<C, EPI, T, false>(p, acc, tm, m0, n0, wm, wn, lane, split);
 #endif
 }

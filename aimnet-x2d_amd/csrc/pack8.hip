@@ -17,8 +17,6 @@ namespace aimx {
 namespace {
 
 typedef int8_t i8x8 __attribute__((ext_vector_type(8)));
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-using dense::floatx4;
 
 constexpr int kNotFinite = 127;
 
@@ -34,28 +32,14 @@ __device__ __forceinline__ int group_exp(uint32_t top) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, int64_t ld, int64_t M, int64_t K, int64_t Kq,
-                                               int8_t* __restrict__ q, int8_t* __restrict__ exps, int vec) {
+                                               int8_t* __restrict__ q, int8_t* __restrict__ exps) {
   const int64_t w = Kq / 8, items = M * w;
   // every thread of a group of 4 stays in the loop as long as the group does (w and the block are
   // multiples of 4)
   for (int64_t it = blockIdx.x * (int64_t)256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
     const int64_t r = it / w, c = (it - r * w) * 8;
     float v[8];
-    const T* p = x + r * ld + c;
-    if (vec && c + 8 <= K) {
-      if constexpr (sizeof(T) == 4) {
-        const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-      } else {
-        const u16x8 a = *reinterpret_cast<const u16x8*>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = dense::from_bf16(a[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c + i < K ? dense::load1(p + i) : 0.f;
-    }
+    dense::load8(x + r * ld + c, K - c, v);
     uint32_t top = 0;  // magnitudes order as their bits, NaN above infinity
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -80,7 +64,7 @@ __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, int64_t 
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_unpack8(const int8_t* __restrict__ q, const int8_t* __restrict__ exps, int64_t M,
-                                                 int64_t K, int64_t Kq, T* __restrict__ y, int64_t ld, int vec) {
+                                                 int64_t K, int64_t Kq, T* __restrict__ y, int64_t ld) {
   const int64_t w = (K + 7) / 8, items = M * w;
   for (int64_t it = blockIdx.x * (int64_t)256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
     const int64_t r = it / w, c = (it - r * w) * 8;
@@ -89,31 +73,10 @@ __global__ __launch_bounds__(256) void k_unpack8(const int8_t* __restrict__ q, c
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = e == kNotFinite ? __uint_as_float(0x7fc00000u) : ldexpf((float)a[i], e);
-    T* p = y + r * ld + c;
-    if (vec && c + 8 <= K) {
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<floatx4*>(p) = floatx4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<floatx4*>(p + 4) = floatx4{v[4], v[5], v[6], v[7]};
-      } else {
-        u16x8 o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = dense::to_bf16(v[i]);
-        *reinterpret_cast<u16x8*>(p) = o;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < K) {
-          if constexpr (sizeof(T) == 4) p[i] = v[i];
-          else p[i] = dense::to_bf16(v[i]);
-        }
-    }
+    dense::store8(y + r * ld + c, K - c, v);
   }
 }
 
-inline int vec_ok(const void* p, int64_t ld, size_t bytes) {
-  return ((uintptr_t)p & 15) == 0 && (ld * (int64_t)bytes) % 16 == 0;
-}
 inline bool args_ok(int32_t dtype, int64_t M, int64_t K, int64_t ld) {
   return (dtype == AIMX_DTYPE_F32 || dtype == AIMX_DTYPE_BF16) && M >= 0 && K >= 1 && ld >= K &&
          M <= ((int64_t)1 << 56) / K;
@@ -133,11 +96,10 @@ extern "C" int aimx_pack8(int32_t dtype, const void* x, int64_t ldx, int64_t M, 
   const int64_t Kq = cdiv(K, 32) * 32;
   const dim3 grid(grid_of(M * (Kq / 8)));
   if (dtype == AIMX_DTYPE_F32)
-    hipLaunchKernelGGL(k_pack8<float>, grid, dim3(256), 0, (hipStream_t)stream, (const float*)x, ldx, M, K, Kq, q, exps,
-                       vec_ok(x, ldx, 4));
+    hipLaunchKernelGGL(k_pack8<float>, grid, dim3(256), 0, (hipStream_t)stream, (const float*)x, ldx, M, K, Kq, q, exps);
   else
     hipLaunchKernelGGL(k_pack8<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t*)x, ldx, M, K, Kq, q,
-                       exps, vec_ok(x, ldx, 2));
+                       exps);
   AIMX_CHECK_LAUNCH();
   return AIMX_OK;
 }
@@ -150,11 +112,10 @@ extern "C" int aimx_unpack8(int32_t dtype, const int8_t* q, const int8_t* exps, 
   const int64_t Kq = cdiv(K, 32) * 32;
   const dim3 grid(grid_of(M * cdiv(K, 8)));
   if (dtype == AIMX_DTYPE_F32)
-    hipLaunchKernelGGL(k_unpack8<float>, grid, dim3(256), 0, (hipStream_t)stream, q, exps, M, K, Kq, (float*)y, ldy,
-                       vec_ok(y, ldy, 4));
+    hipLaunchKernelGGL(k_unpack8<float>, grid, dim3(256), 0, (hipStream_t)stream, q, exps, M, K, Kq, (float*)y, ldy);
   else
     hipLaunchKernelGGL(k_unpack8<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, q, exps, M, K, Kq, (uint16_t*)y,
-                       ldy, vec_ok(y, ldy, 2));
+                       ldy);
   AIMX_CHECK_LAUNCH();
   return AIMX_OK;
 }

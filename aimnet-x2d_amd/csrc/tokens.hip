@@ -18,55 +18,60 @@ namespace aimx {
 namespace {
 
 using dense::floatx4;
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
-// 16 bytes of a row, or one element where rows are not 16-byte aligned
-template <typename T, int VEC>
+// 16 bytes of a row from p, `left` elements of which exist
+template <typename T>
 struct Cols {
-  float v[VEC];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (VEC == 1) {
-      v[0] = dense::load1(p);
-    } else if constexpr (sizeof(T) == 4) {
-      const floatx4 a = *reinterpret_cast<const floatx4*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = a[i];
+  static constexpr int kVec = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(kVec)));
+  typedef T vece __attribute__((ext_vector_type(kVec), aligned(sizeof(T))));
+  vec v;
+  __device__ __forceinline__ void load(const T* p, int64_t left) {
+    if (left >= kVec) {
+      v = *reinterpret_cast<const vece*>(p);
     } else {
-      const u16x8 a = *reinterpret_cast<const u16x8*>(p);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = dense::from_bf16(a[i]);
+      for (int e = 0; e < kVec; ++e) v[e] = e < left ? p[e] : (T)0;
     }
   }
-  __device__ __forceinline__ void store(T* p, float scale) const {
-    if constexpr (VEC == 1) {
-      if constexpr (sizeof(T) == 4) *p = v[0] * scale;
-      else *p = dense::to_bf16(v[0] * scale);
-    } else if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<floatx4*>(p) = floatx4{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(T) == 4) return v[e];
+    else return dense::from_bf16(v[e]);
+  }
+  __device__ __forceinline__ void set(int e, float f) {
+    if constexpr (sizeof(T) == 4) v[e] = f;
+    else v[e] = dense::to_bf16(f);
+  }
+  __device__ __forceinline__ void store(T* p, int64_t left) const {
+    if (left >= kVec) {
+      *reinterpret_cast<vece*>(p) = v;
     } else {
-      u16x8 o;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = dense::to_bf16(v[i] * scale);
-      *reinterpret_cast<u16x8*>(p) = o;
+      for (int e = 0; e < kVec; ++e)
+        if (e < left) p[e] = v[e];
     }
   }
 };
+template <typename T>
+__device__ __forceinline__ void store1(T* p, float f) {
+  if constexpr (sizeof(T) == 4) *p = f;
+  else *p = dense::to_bf16(f);
+}
 
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void k_token_gather(const int64_t* __restrict__ index, int64_t n,
                                                       const T* __restrict__ table, int64_t V, int64_t D, float scale,
                                                       T* __restrict__ out) {
-  const int64_t w = D / VEC, items = n * w;
+  constexpr int kVec = Cols<T>::kVec;
+  const int64_t w = (D + kVec - 1) / kVec, items = n * w;
   for (int64_t it = blockIdx.x * (int64_t)256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
-    const int64_t i = it / w, c = (it - i * w) * VEC, v = index[i];
-    Cols<T, VEC> a;
-    if (v >= 0 && v < V) {
-      a.load(table + v * D + c);
-    } else {
+    const int64_t i = it / w, c = (it - i * w) * kVec, v = index[i];
+    const bool ok = v >= 0 && v < V;
+    Cols<T> a;
+    a.load(table + (ok ? v : 0) * D + c, ok ? D - c : 0);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) a.v[e] = 0.f;
-    }
-    a.store(out + i * D + c, scale);
+    for (int e = 0; e < kVec; ++e) a.set(e, a.get(e) * scale);
+    a.store(out + i * D + c, D - c);
   }
 }
 
@@ -214,7 +219,7 @@ struct Runs {
   int64_t n, V, D, ldd, seg, segs;
   int64_t slices;  // column slices of a row
   int32_t group;   // lanes of a slice
-  int64_t ldp;     // D rounded up to 4
+  int64_t ldp;     // D rounded up to 8
   float* head;     // [segs][ldp]: the part of a run that began before the segment
   float* tail;     // [segs][ldp]: the part of a run that goes on behind it and began inside
   float scale;
@@ -222,8 +227,9 @@ struct Runs {
 
 constexpr int kAhead = 8;  // rows in flight
 
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void k_token_runs(const Runs a, const T* __restrict__ dy, T* __restrict__ dtable) {
+  constexpr int VEC = Cols<T>::kVec;
   const int64_t worker = (blockIdx.x * (int64_t)256 + threadIdx.x) / a.group;
   const int64_t seg = worker / a.slices;
   const int64_t c = ((worker - seg * a.slices) * a.group + threadIdx.x % a.group) * VEC;
@@ -235,13 +241,13 @@ __global__ __launch_bounds__(256) void k_token_runs(const Runs a, const T* __res
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
   for (int64_t p = p0; p < p1; p += kAhead) {
-    Cols<T, VEC> row[kAhead];
+    Cols<T> row[kAhead];
     uint32_t key[kAhead + 1];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int64_t q = min(p + j, p1 - 1);
       key[j] = a.key[q];
-      row[j].load(dy + (int64_t)a.id[q] * a.ldd + c);
+      row[j].load(dy + (int64_t)a.id[q] * a.ldd + c, a.D - c);
     }
     key[kAhead] = p + kAhead < a.n ? a.key[p + kAhead] : none + 1;
 #pragma unroll
@@ -249,7 +255,7 @@ __global__ __launch_bounds__(256) void k_token_runs(const Runs a, const T* __res
       const int64_t q = p + j;
       if (q < p1) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += row[j].v[e];
+        for (int e = 0; e < VEC; ++e) acc[e] += row[j].get(e);
         // the key behind q: of the next row here, or across the segment's end
         uint32_t next = key[j + 1];
         if (q + 1 == p1) next = p1 < a.n ? a.key[p1] : none + 1;
@@ -259,12 +265,12 @@ __global__ __launch_bounds__(256) void k_token_runs(const Runs a, const T* __res
             if (from_before || !ends) {
               float* part = (from_before ? a.head : a.tail) + seg * a.ldp + c;
 #pragma unroll
-              for (int e = 0; e < VEC; ++e) part[e] = acc[e];
+              for (int e = 0; e < VEC; ++e) part[e] = acc[e];  // ldp is a multiple of 8
             } else {
-              Cols<T, VEC> o;
+              Cols<T> o;
 #pragma unroll
-              for (int e = 0; e < VEC; ++e) o.v[e] = acc[e];
-              o.store(dtable + (int64_t)key[j] * a.D + c, a.scale);
+              for (int e = 0; e < VEC; ++e) o.set(e, acc[e] * a.scale);
+              o.store(dtable + (int64_t)key[j] * a.D + c, a.D - c);
             }
           }
           from_before = false;
@@ -306,11 +312,7 @@ __global__ __launch_bounds__(256) void k_token_join(const Runs a, T* __restrict_
       for (int j = 0; j < parts; ++j) s += at(a.head, seg + 1 + j);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < a.D) {
-          Cols<T, 1> o;
-          o.v[0] = s[e];
-          o.store(dtable + (int64_t)key * a.D + c + e, a.scale);
-        }
+        if (c + e < a.D) store1(dtable + (int64_t)key * a.D + c + e, s[e] * a.scale);
     }
   }
   __syncthreads();
@@ -348,11 +350,10 @@ __global__ __launch_bounds__(256) void k_token_join(const Runs a, T* __restrict_
     __syncthreads();
     const int64_t col = blockIdx.y * (int64_t)64 + threadIdx.x;
     if (threadIdx.x < 64 && col < a.D) {
-      Cols<T, 1> o;
-      o.v[0] = 0.f;
+      float f = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o.v[0] += part[i][threadIdx.x];
-      o.store(dtable + (int64_t)key * a.D + col, a.scale);
+      for (int i = 0; i < 16; ++i) f += part[i][threadIdx.x];
+      store1(dtable + (int64_t)key * a.D + col, f * a.scale);
     }
     __syncthreads();
   }
@@ -390,7 +391,7 @@ Layout layout(char* base, int64_t n, int64_t V, int64_t D) {
     l.s.id[i] = (uint32_t*)take((size_t)n * 4);
   }
   l.s.hist = (int32_t*)take((size_t)l.s.chunks * 256 * 4);
-  l.r.ldp = (D + 3) / 4 * 4;
+  l.r.ldp = (D + 7) / 8 * 8;
   l.r.head = (float*)take((size_t)l.r.segs * l.r.ldp * 4);
   l.r.tail = (float*)take((size_t)l.r.segs * l.r.ldp * 4);
   l.bytes = used;
@@ -401,13 +402,8 @@ inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename T>
 int gather(const int64_t* index, int64_t n, const T* table, int64_t V, int64_t D, float scale, T* out, hipStream_t st) {
-  constexpr int kVec = 16 / sizeof(T);
-  const bool vec = D % kVec == 0 && al16(table) && al16(out);
-  const dim3 grid((unsigned)std::min<int64_t>(cdiv(n * (vec ? D / kVec : D), 256), 32768));
-  if (vec)
-    hipLaunchKernelGGL((k_token_gather<T, kVec>), grid, dim3(256), 0, st, index, n, table, V, D, scale, out);
-  else
-    hipLaunchKernelGGL((k_token_gather<T, 1>), grid, dim3(256), 0, st, index, n, table, V, D, scale, out);
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(n * cdiv(D, Cols<T>::kVec), 256), 32768));
+  hipLaunchKernelGGL((k_token_gather<T>), grid, dim3(256), 0, st, index, n, table, V, D, scale, out);
   AIMX_CHECK_LAUNCH();
   return AIMX_OK;
 }
@@ -445,16 +441,13 @@ int grad(const int64_t* index, int64_t n, const T* dy, int64_t ldd, int64_t V, i
   r.D = D;
   r.ldd = ldd;
   r.scale = scale;
-  constexpr int kVec = 16 / sizeof(T);
-  const bool vec = D % kVec == 0 && ldd % kVec == 0 && al16(dy) && al16(dtable);
-  const int64_t cols = cdiv(D, vec ? kVec : 1);
+  const int64_t cols = cdiv(D, Cols<T>::kVec);
   r.group = 1;
   while (r.group < 64 && r.group < cols) r.group *= 2;
   r.slices = cdiv(cols, r.group);
   const int64_t blocks = cdiv(r.segs * r.slices * r.group, 256);
   if (blocks > INT32_MAX) return AIMX_EARG;
-  if (vec) hipLaunchKernelGGL((k_token_runs<T, kVec>), dim3((unsigned)blocks), dim3(256), 0, st, r, dy, dtable);
-  else hipLaunchKernelGGL((k_token_runs<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, r, dy, dtable);
+  hipLaunchKernelGGL((k_token_runs<T>), dim3((unsigned)blocks), dim3(256), 0, st, r, dy, dtable);
   AIMX_CHECK_LAUNCH();
   if (r.segs > 1) {
     hipLaunchKernelGGL((k_token_join<T>), dim3((unsigned)cdiv(r.segs - 1, 16), (unsigned)cdiv(D, 64)), dim3(256), 0, st, r,
