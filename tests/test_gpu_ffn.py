@@ -256,3 +256,111 @@ def test_checkpoint_with_a_diverged_group_gives_nan():
     w = torch.randn(16, 64, device=DEV, requires_grad=True)
     g, = torch.autograd.grad(ops.dense(x, w, checkpoint8=True).sum(), w)
     assert torch.isnan(g[:, :32]).all() and torch.isfinite(g[:, 32:]).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# Long tensors, captured graphs, streams
+# ---------------------------------------------------------------------------------------------
+def _graph(fn, warm=3):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(warm):
+            fn()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = fn()
+    return g, out
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("halves,act,ckpt,M,K,N", [(2, "silu", False, 700, 128, 96), (1, "gelu", True, 333, 77, 45),
+                                                   (1, None, False, 40, 4096, 48)])
+def test_captured_passes_replay(halves, act, ckpt, M, K, N, dtype):
+    """Forward and gradients captured once; each replay on new inputs equals the eager pass bit for bit, with eager
+    passes of the same operator between the replays. Two graphs share nothing."""
+    ops = _ops()
+    x, ws, bs, _, dy = [t.to(DEV) if torch.is_tensor(t) else [v.to(DEV) for v in t] if t else t
+                        for t in _make(M, K, N, dtype, halves)]
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, *ws, *bs)]
+        if halves == 2:
+            y = ops.gated_linear(*leaves, act=act, checkpoint8=ckpt)
+        else:
+            y = ops.dense(*leaves, act=act, checkpoint8=ckpt)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    graphs = [_graph(step) for _ in range(2)]
+    for k in range(3):
+        x.copy_(torch.randn(M, K, device=DEV))
+        dy.copy_(torch.randn(M, N, device=DEV))
+        want = [t.clone() for t in step()]
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_same_bits_every_time():
+    """Split sums and column sums are joined in a fixed order."""
+    for dtype in (F32, BF16):
+        args = _make(5000, 200, 72, dtype, 2)
+        first = _run(*args[:3], "silu", None, args[4])
+        for _ in range(3):
+            again = _run(*args[:3], "silu", None, args[4])
+            assert all(torch.equal(first[k], again[k]) for k in first)
+
+
+@pytest.mark.parametrize("K", [512, 520])
+def test_rows_past_2_31_elements(K):
+    """4.2 million rows, read in place (512 columns) and staged (520): the last rows equal the same rows alone."""
+    ops = _ops()
+    M = 4_200_003
+    x = torch.empty(M, K, dtype=BF16, device=DEV)
+    x[-70:] = torch.randn(70, K, device=DEV)
+    x[:70] = torch.randn(70, K, device=DEV)
+    x[70:-70] = 0.25
+    w, b = torch.randn(24, K, device=DEV, dtype=BF16), torch.randn(24, device=DEV, dtype=BF16)
+    y = ops.gated_linear(x, w, w * 0.5, b, b)
+    for rows in (slice(0, 70), slice(M - 70, M)):
+        assert torch.equal(y[rows], ops.gated_linear(x[rows].clone(), w, w * 0.5, b, b))
+    assert torch.equal(y[M // 2], y[M // 2 + 1])
+    p = ops.unpack8(ops.pack8(x))
+    for rows in (slice(0, 70), slice(M - 70, M)):
+        assert torch.equal(p[rows], ops.unpack8(ops.pack8(x[rows].clone())))
+    with pytest.raises(Exception, match="2\\^22 rows"):
+        ops.dense(x, w.requires_grad_())
+
+
+def test_gradients_of_two_million_rows():
+    """Weight and bias gradients over 2^21 + 5 rows: ones in some rows, zeros elsewhere, so the sums are exact."""
+    ops = _ops()
+    M, K, N = 2 ** 21 + 5, 40, 24
+    x, dy = torch.zeros(M, K, dtype=BF16, device=DEV), torch.zeros(M, N, dtype=BF16, device=DEV)
+    hot = torch.arange(0, M, 16411, device=DEV)
+    x[hot], dy[hot] = 1, 2
+    x[-1], dy[-1] = 1, 2
+    w, b = torch.zeros(N, K, dtype=BF16, device=DEV, requires_grad=True), torch.zeros(N, dtype=BF16, device=DEV,
+                                                                                      requires_grad=True)
+    n = int((dy[:, 0] != 0).sum())
+    dw, db = torch.autograd.grad(ops.dense(x, w, b), [w, b], dy)
+    want = torch.full((), 2.0 * n).to(BF16)
+    assert (dw.cpu() == want).all() and (db.cpu() == want).all()
+
+
+def test_calls_on_other_streams():
+    ops = _ops()
+    x, ws, bs, _, dy = _make(900, 130, 70, F32, 2)
+    want = _run(x, ws, bs, "silu", None, dy)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(_run(x, ws, bs, "silu", None, dy))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g[k], want[k]) for g in got for k in want)

@@ -237,3 +237,21 @@ def test_two_streams_at_once():
                 got.append((ops.gated_linear(x, w, u), torch.autograd.grad(ops.embedding(index, table), table, dy)[0]))
     torch.cuda.synchronize()
     assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
+
+
+def test_table_past_2_31_elements():
+    ops = _ops()
+    V, D = 2 ** 22 + 3, 520
+    table = torch.zeros(V, D, dtype=BF16, device=DEV)
+    rows = torch.tensor([0, 5, V - 1, V // 2, V - 1, 0], device=DEV)
+    table[rows] = torch.randn(6, D, device=DEV).to(BF16)
+    table.requires_grad_()
+    y = ops.embedding(rows, table, 2.0)
+    assert torch.equal(y, table[rows] * 2)
+    dy = torch.randn(6, D, device=DEV).to(BF16)
+    g, = torch.autograd.grad(y, table, dy)
+    for v in (0, 5, V // 2, V - 1):
+        want = (dy[rows == v].float().sum(0) * 2).to(BF16)
+        assert torch.equal(g[v], want)
+    g[rows] = 0
+    assert not g.view(-1, 4).any(dim=0).any()
