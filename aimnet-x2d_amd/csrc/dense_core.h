@@ -683,8 +683,8 @@ inline Plan pick(const Shape* shapes, int n, int64_t M, int64_t columns, int64_t
       const double part = rest == 0 ? 0. : s.per_cu == 1 ? 1. : std::max(0.47, 0.2 + 0.8 * (double)rest / (double)slots);
       const double rounds = (double)(all / slots) + part;
       double t = rounds * ((double)cdiv(steps, k) * s.step + s.end);
-      // the slabs are written and read again, about 4.5 TB/s, by one more launch
-      if (k > 1) t += 5. + (double)(6 * k + 4) * (double)M * (double)columns / 4.5e6;
+      // one more launch reads the slabs, which the caches hold in part: 8 of 4 MB in 6.8 us
+      if (k > 1) t += 4. + (double)(3 * k + 2) * (double)M * (double)columns / 4.5e6;
       if (t < least) least = t, best = Plan{s.tile, (int)k, s.rows};
       if (all > 16 * slots) break;
     }
