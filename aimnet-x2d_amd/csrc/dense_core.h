@@ -400,8 +400,8 @@ __device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN]
     if (whole) return shift > 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : d.get();
     return d.get((int)min(shift, (int64_t)4));
   };
-  // rows whose operands are in flight together, 16 registers of them
-  constexpr int kMost = 16 / sizeof(T) / FH, kAhead = kMost < 1 ? 1 : kMost < C::FM ? kMost : C::FM;
+  // rows whose operands are in flight together, 32 registers of them
+  constexpr int kMost = 32 / sizeof(T) / FH, kAhead = kMost < 1 ? 1 : kMost < C::FM ? kMost : C::FM;
 #pragma unroll
   for (int j0 = 0; j0 < C::FM; j0 += kAhead) {
     Raw4<T> d[kAhead][FH];
