@@ -13,8 +13,8 @@
 // would be 335 MB written and read again. fp32 tensors keep them: their product costs six times as much.
 //
 // Roundings to fewer bits: y, dx, dW and db once, to the tensors' type. bf16 tensors: dP / dG / dU are
-// rounded to bf16 for the matrix instructions (their sums for db are not); with the result's own rounding
-// that makes sqrt(2) of the error of rounding the result alone. fp32 tensors: none.
+// rounded to bf16 for the matrix instructions (their sums for db are not), unless they are few; with the result's
+// own rounding that makes sqrt(2) of the error of rounding the result alone. fp32 tensors: none.
 #include "dense_core.h"
 
 namespace aimx {
@@ -236,7 +236,7 @@ void product(Ctx& c, Carve& ws, Problem p, int pa, int pb, int epi, int across, 
   if (p.M == 0) return;
   const bool one = pa == 1 && pb == 1;
   const int halves = epi == kGated || epi == kGatedGrad ? 2 : 1;
-  const Plan t = one ? plan_one(p.M, p.N * halves, p.K, epi == kPlain) : plan_split(p.M, p.N * halves, p.K, epi == kPlain);
+  const Plan t = one ? plan_one(p.M, p.N * halves, p.K, epi == kPlain) : plan_split(p.M, p.N * halves, p.K, epi == kPlain, fp32);
   p.splits = t.splits;
   if (t.splits > 1) p.slab = ws.take<float>((int64_t)t.splits * p.M * p.N);
   if (c.dry || c.rc) return;
@@ -244,7 +244,7 @@ void product(Ctx& c, Carve& ws, Problem p, int pa, int pb, int epi, int across, 
   p.np = up64(p.N);
   if (p.k_half == 0) p.k_half = p.K;
   if (p.y_rows == 0) p.y_rows = p.y_valid = p.M;
-  c.rc = one ? launch_one(p, t.tile, epi, across, fp32, c.st) : launch_split(p, t.tile, pa, pb, epi, across, c.st);
+  c.rc = one ? launch_one(p, t.tile, epi, across, fp32, c.st) : launch_split(p, t.tile, pa, pb, epi, across, fp32, c.st);
   if (c.rc || t.splits == 1) return;
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(p.M * cdiv(p.N, 4), 256), 16384));
   if (fp32) hipLaunchKernelGGL(k_reduce_slabs<float>, grid, dim3(256), 0, c.st, p);
@@ -347,7 +347,11 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
   const int64_t M = d->M, N = d->N, K = d->K, H = d->halves, Np = up64(N);
   const bool has_dw = g->dw[0] != nullptr, has_db = g->db[0] != nullptr, has_dx = g->dx != nullptr;
   const bool again = d->act >= 0 && !d->pre;  // the values before the activation are computed again
-  const int px = d->x ? k.planes : 1;
+  // Where the gradient before the activation holds few values, the error of rounding them to bf16 does not average out
+  // in dx and dW (1.5 times that of rounding the results at one row of 32): three planes of it cost nothing
+  // there. The forward's values then come as fp32 first.
+  const bool fine = !k.fp32 && d->act >= 0 && M * H * N <= 65536;
+  const int px = d->x ? k.planes : 1, pd = fine ? 3 : k.planes;
   Segments same{}, eight{};
   Operand x{}, w{}, rows{};
   if (has_dw || again) x = operand_x(d, k, ws, again, same, eight);
@@ -359,7 +363,15 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
   const int64_t plane = M * H * Np;
   const float* sums = nullptr;
   int64_t parts = 0;
-  if (again) {
+  const float* pre = d->pre;
+  if (fine && again) {
+    Problem p = forward_problem(d, x, w);
+    p.y = ws.take<uint16_t>(M * N);
+    p.ldy = N;
+    pre = p.pre = ws.take<float>(M * H * ((N + 7) / 8 * 8));
+    product(c, ws, p, 1, 1, H == 2 ? kGated : kPlain, kNone, false);
+  }
+  if (again && !fine) {
     uint16_t* t = ws.take<uint16_t>(plane * k.planes);
     rows = {t, nullptr, H * Np, plane, M, H * Np};
     Problem p = forward_problem(d, x, w);
@@ -367,7 +379,7 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     p.ldr = g->ldd;
     p.rows = t;
     p.rows_plane = plane;
-    const Plan at = (px == 1 && k.planes == 1) ? plan_one(M, N * H, p.K, false) : plan_split(M, N * H, p.K, false);
+    const Plan at = (px == 1 && k.planes == 1) ? plan_one(M, N * H, p.K, false) : plan_split(M, N * H, p.K, false, k.fp32);
     parts = cdiv(M, at.rows) * kWavesM;
     if (has_db) sums = p.sums = ws.take<float>(parts * H * N);
     product(c, ws, p, px, k.planes, H == 2 ? kGatedGrad : kDenseGrad, kNone, k.fp32);
@@ -379,12 +391,12 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     a.N = N;
     a.Np = Np;
     a.N8 = (N + 7) / 8 * 8;
-    a.pre = d->act >= 0 ? d->pre : nullptr;
+    a.pre = d->act >= 0 ? pre : nullptr;
     a.act = d->act;
     if (d->act < 0 && in_place(k, g->dy, g->ldd, N, has_dx)) {
       rows = {(const uint16_t*)g->dy, nullptr, g->ldd, 0, M, N};
     } else if (has_dx || has_dw) {
-      a.rows = ws.take<uint16_t>(plane * k.planes);
+      a.rows = ws.take<uint16_t>(plane * pd);
       a.plane = plane;
       rows = {a.rows, nullptr, H * Np, plane, M, H * Np};
     }
@@ -392,6 +404,7 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     if (has_db) sums = a.sums = ws.take<float>(parts * H * N);
     if (!c.dry && !c.rc && M > 0 && (a.rows || a.sums)) {
       if (Np / 64 * parts > INT32_MAX) c.rc = AIMX_EARG;
+      else if (!k.fp32 && fine) dpre_go<uint16_t, 3>(c, a, (int)H);
       else if (!k.fp32) dpre_go<uint16_t, 1>(c, a, (int)H);
       else if (k.planes == 3) dpre_go<float, 3>(c, a, (int)H);
       else dpre_go<float, 1>(c, a, (int)H);
@@ -418,7 +431,7 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     p.y = g->dx;
     p.ldy = g->lddx;
     p.act = AIMX_ACT_NONE;
-    product(c, ws, p, k.planes, k.planes, kPlain, kB, k.fp32);
+    product(c, ws, p, pd, k.planes, kPlain, kB, k.fp32);
   }
   if (has_dw) {
     Problem p{};
@@ -433,7 +446,7 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     p.y_rows = H == 2 ? Np : N;
     p.y_valid = N;
     p.act = AIMX_ACT_NONE;
-    product(c, ws, p, k.planes, px, kPlain, kBoth, k.fp32);
+    product(c, ws, p, pd, px, kPlain, kBoth, k.fp32);
   }
 }
 

@@ -692,12 +692,12 @@ inline Plan pick(const Shape* shapes, int n, int64_t M, int64_t columns, int64_t
   return best;
 }
 Plan plan_one(int64_t M, int64_t columns, int64_t K, bool may_split);
-Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split);
-// Launchers (dense_bf16.hip: one plane a side; dense_split.hip: three planes on one side or both, fp32 tensors).
+Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split, bool fp32);
+// Launchers (dense_bf16.hip: one plane a side; dense_split.hip: three planes on one side or both).
 // epi: kPlain, kGated, kDenseGrad or kGatedGrad. p.splits > 1 (kPlain): the partial sums go to p.slab, and the
 // caller's reduction applies the epilogue.
 int launch_one(const Problem& p, int tile, int epi, int across, bool fp32, hipStream_t st);
-int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, hipStream_t st);
+int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, bool fp32, hipStream_t st);
 
 template <typename C, int EPI, int ACROSS, typename T>
 int launch_config(const Problem& p, hipStream_t st) {

@@ -1,4 +1,5 @@
-// Three-plane products: fp32 tensors at fp32 accuracy.
+// Three-plane products: fp32 tensors at fp32 accuracy, and the small bf16 backward products whose first operand, the
+// gradient before the activation, keeps fp32's accuracy.
 #include "dense_core.h"
 
 namespace aimx {
@@ -41,14 +42,21 @@ int go(const Problem& p, int pa, int pb, int epi, int across, hipStream_t st) {
 }  // namespace
 
 // At 9186 rows, 256 -> 2 x 683: 3168 small tiles 67 us, 792 middle ones 72; at 20480 rows, 512 -> 2 x 2048: 745 and 595.
-Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split) {
+Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split, bool fp32) {
   static const Shape shapes[] = {{0, 128, 128, 32, 1, 1.1, 9.}, {1, 64, 64, 32, 3, 1.5, 4.}, {2, 256, 128, 32, 1, 1.95, 12.}};
+  if (!fp32) return pick(shapes + 1, 1, M, columns, K, may_split);
   const int64_t force = tune_i64("AIMX_DENSE_SPLIT_TILE", -1);
   if (force >= 0) return pick(shapes + force, 1, M, columns, K, may_split);
   return pick(shapes, 3, M, columns, K, may_split);
 }
 
-int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, hipStream_t st) {
+int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, bool fp32, hipStream_t st) {
+  if (!fp32) {
+    if (pa != 3 || pb != 1 || epi != kPlain || across == kNone) return AIMX_EARG;
+    using C = Small<3, 1>;
+    if (p.splits > 1) return across == kB ? launch_config<C, kSlab, kB, float>(p, st) : launch_config<C, kSlab, kBoth, float>(p, st);
+    return across == kB ? launch_config<C, kPlain, kB, uint16_t>(p, st) : launch_config<C, kPlain, kBoth, uint16_t>(p, st);
+  }
   if (tile == 2) return go<Large>(p, pa, pb, epi, across, st);
   return tile == 0 ? go<Medium>(p, pa, pb, epi, across, st) : go<Small>(p, pa, pb, epi, across, st);
 }

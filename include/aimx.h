@@ -599,7 +599,8 @@ int aimx_pad_batch(const AimxPadBatch* p, aimx_stream_t stream);
  * aimx_dense_backward: dy [M, N] -> dx [M, K], dw [N, K] (contiguous), db [N], each written when its
  * pointer is given (dw and db of both halves or of neither). It reads x, w, pre of d (b only where pre is
  * NULL); with x NULL it runs on the 8-bit form of x (q, qexp: aimx_pack8), whose values it takes for x also
- * where it computes pre again. bf16 tensors: the gradient before the activation is rounded to bf16 once.
+ * where it computes pre again. bf16 tensors: the gradient before the activation is rounded to bf16 once where
+ * it holds more than 65536 values.
  * M = 0: dw and db are zero-filled.
  * ------------------------------------------------------------------------------------------ */
 #define AIMX_DTYPE_F32 0

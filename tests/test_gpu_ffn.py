@@ -119,6 +119,19 @@ def test_fp32_is_fp32():
         assert (y - ref).norm() / ref.norm() < K ** 0.5 * 2.0 ** -24
 
 
+def test_few_bf16_values_round_once():
+    """One row: dW is an outer product and dx one row, so a rounding of the gradient before the activation would show
+    whole. Each result is within one rounding to bf16 (2^-8) of the 64-bit value, and fp32 sums' error."""
+    for halves, M, K, N in ((2, 1, 32, 32), (1, 3, 50, 40), (2, 40, 96, 70)):
+        x, ws, bs, _, dy = _make(M, K, N, BF16, halves)
+        got = _run(x, ws, bs, "silu", None, dy)
+        val, tol = product64(x, ws, bs, "silu", None, dy, F32)
+        for k, v in got.items():
+            err = (v.double().cpu() - val[k]).abs()
+            # the hardware exp2 and reciprocal of the 16-bit forward are off by 2^-18 at most (y only)
+            assert (err <= tol[k] * 2 + 2.0 ** -8 * val[k].abs() * (1 + 2.0 ** -6) + 2.0 ** -18 * val[k].abs()).all(), k
+
+
 def test_magnitudes_fp32():
     """Exponents from 2^-60 to 2^60 in one product, and values at the end of the range in either operand."""
     g = torch.Generator().manual_seed(3)
