@@ -10,6 +10,11 @@
 // crosses segments leaves a partial row per segment, and the segment it begins in adds them in order. So no
 // atomics touch a float, the sums are fp32 and the same in every run, and a token with half of all items costs
 // no more than its share of segments.
+//
+// 65536 tokens in a 32000 x 512 bf16 table: the lookup 18 us (67 MB written, 4.4 TB/s with the rows read), the zero fill
+// 7.5, the sort's two passes of three launches 31 (latency: 64 workgroups), the runs 18 to 24 (90 MB), their join 10.
+// A group of 32 rows a segment: fewer leave more runs to join, more leave too few groups to hide the scattered
+// rows' latency (kAhead rows are in flight in each).
 #include <algorithm>
 
 #include "dense_core.h"
