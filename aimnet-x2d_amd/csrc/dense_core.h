@@ -278,8 +278,8 @@ struct Loader {
   static constexpr int kWaves = C::kThreads / kWave;
   static constexpr int kLoads = ROWS * C::U / kWave / kWaves;  // of a wave, per plane
   static constexpr int UR = ROWS / 8;                          // units of a k row, across
-  // rows (across: of k) that all waves' j-th loads cover: the permutations repeat after as many, so a lane has one
-  // offset and load j adds a scalar
+  // rows (across: of k) that all waves' j-th loads cover: the permutations repeat after as many, so a lane keeps one
+  // offset and load j adds to it
   static constexpr int kStep = kWaves * (T ? kWave / UR : C::kRowsPerLoad);
   static_assert(ROWS * C::U % (kWave * kWaves) == 0, "every wave issues whole loads");
   static_assert(kStep % (T ? 16 : 8) == 0, "the permutations repeat");
@@ -316,6 +316,8 @@ struct Loader {
     }
   }
 
+  // The whole offset goes where the descriptor's range is checked against it: a scalar offset is subtracted from the
+  // range first, which wraps where fewer bytes are left than it skips (the rows and k past a matrix's end).
   __device__ __forceinline__ void load(char* base, int64_t step, int64_t k_half) const {
     typedef __attribute__((address_space(3))) void lds_void;
     const uint32_t ld2 = (uint32_t)o.ld * 2;
@@ -332,7 +334,8 @@ struct Loader {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(
-              d, (lds_void*)(base + (q * ROWS * C::U + (j * kWaves + wave) * kWave) * 16), 16, off, j * kStep * ld2, 0, 0);
+              d, (lds_void*)(base + (q * ROWS * C::U + (j * kWaves + wave) * kWave) * 16), 16, off + j * kStep * ld2, 0, 0,
+              0);
       }
     } else {
       const uint32_t kb = (uint32_t)(step * C::BK * 2);
@@ -343,8 +346,8 @@ struct Loader {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           lds_void* dst = (lds_void*)(base + (q * ROWS * C::U + (j * kWaves + wave) * kWave) * 16);
-          if (half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, off, at, 0, 0);
-          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, off, at, 0, 0);
+          if (half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, off + at, 0, 0, 0);
+          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, off + at, 0, 0, 0);
         }
       }
     }
