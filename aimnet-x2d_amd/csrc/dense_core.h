@@ -316,8 +316,9 @@ struct Loader {
     }
   }
 
-  // The whole offset goes where the descriptor's range is checked against it: a scalar offset is subtracted from the
-  // range first, which wraps where fewer bytes are left than it skips (the rows and k past a matrix's end).
+  // Rows are skipped by the offset that the descriptor's range is checked against: a scalar offset is subtracted from the
+  // range first, which would wrap where fewer bytes are left than it skips. Along the rows the scalar is k, which
+  // stays inside the first row (0 where the tile has no row).
   __device__ __forceinline__ void load(char* base, int64_t step, int64_t k_half) const {
     typedef __attribute__((address_space(3))) void lds_void;
     const uint32_t ld2 = (uint32_t)o.ld * 2;
@@ -338,16 +339,16 @@ struct Loader {
               0);
       }
     } else {
-      const uint32_t kb = (uint32_t)(step * C::BK * 2);
+      const uint32_t kb = row0 < o.rows ? (uint32_t)(step * C::BK * 2) : 0u;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int half = HALVES == 1 ? 0 : ((j * kStep + wave * C::kRowsPerLoad) / (WT / 2)) & 1;
-        const uint32_t at = kb + source_row(j * kStep) * ld2;
+        const uint32_t at = off + source_row(j * kStep) * ld2;
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           lds_void* dst = (lds_void*)(base + (q * ROWS * C::U + (j * kWaves + wave) * kWave) * 16);
-          if (half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, off + at, 0, 0, 0);
-          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, off + at, 0, 0, 0);
+          if (half == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][0], dst, 16, at, kb, 0, 0);
+          else __builtin_amdgcn_raw_ptr_buffer_load_lds(r[q][HALVES - 1], dst, 16, at, kb, 0, 0);
         }
       }
     }
