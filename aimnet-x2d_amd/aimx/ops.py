@@ -1277,9 +1277,13 @@ class _DenseFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         import ctypes
+        # grad mode is on here only under create_graph. The gradients depend on x and the weights, so a result
+        # without a graph would drop second-order terms unseen (once_differentiable marks it only where dy itself
+        # requires grad); an edge to x would keep alive what checkpoint8 frees.
+        if torch.is_grad_enabled():
+            raise _lib.AimxError("aimx.dense, gated_linear: no second derivatives (backward with create_graph=True)")
         lib = _lib.load()
         kept, exps, pre, *rest = ctx.saved_tensors
         ws, bs = rest[:ctx.halves], rest[ctx.halves:]
@@ -1361,7 +1365,8 @@ def _dense_apply(what, x, ws, bs, res, act, checkpoint8):
 def dense(x, w, b=None, act=None, residual=None, checkpoint8=False):
     """y = act(x w^T + b) + residual in one kernel: x [..., n_in], w [n_out, n_in], b [n_out] or None, act None
     or an activation name, residual [..., n_out] or None; all fp32 or all bf16. fp32 at fp32 accuracy
-    (bf16 operands inside torch.autocast, as linear()). Differentiable in every tensor.
+    (bf16 operands inside torch.autocast, as linear()). Differentiable once in every tensor; a backward with
+    create_graph=True raises.
     checkpoint8=True: what is kept for the backward is x in 8 bits (pack8: 33/32 bytes a value) instead of x
     (fp32: and the values before the activation); the gradients are those at the x that the bits stand for."""
     kind = _dense_checks("dense", x, [w], [b], act, residual)
@@ -1370,8 +1375,8 @@ def dense(x, w, b=None, act=None, residual=None, checkpoint8=False):
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", checkpoint8=False):
     """h = act(x w_gate^T + b_gate) * (x w_up^T + b_up): both projections, the activation and the product in one
-    kernel. x [..., n_in], weights [n_out, n_in], biases [n_out] or None (both or neither). Types, autocast
-    and checkpoint8 as in dense()."""
+    kernel. x [..., n_in], weights [n_out, n_in], biases [n_out] or None (both or neither). Types, autocast,
+    derivatives and checkpoint8 as in dense()."""
     if act is None:
         raise _lib.AimxError("aimx.gated_linear: act names the gate's activation")
     if (b_gate is None) != (b_up is None):

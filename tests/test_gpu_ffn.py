@@ -364,6 +364,22 @@ def test_gradients_of_two_million_rows():
     assert (dw.cpu() == want).all() and (db.cpu() == want).all()
 
 
+def test_one_weight_twice_and_no_second_derivative():
+    ops = _ops()
+    x = torch.randn(30, 40, device=DEV, requires_grad=True)
+    w = torch.randn(50, 40, device=DEV, requires_grad=True)
+    dy = torch.randn(30, 50, device=DEV)
+    a, b = w.detach().requires_grad_(), w.detach().requires_grad_()
+    ga, gb = torch.autograd.grad(ops.gated_linear(x, a, b), [a, b], dy)
+    assert torch.equal(torch.autograd.grad(ops.gated_linear(x, w, w), w, dy)[0], ga + gb)
+    # refused where the first gradient is asked for: detached, it would drop the second-order terms unseen
+    for call in (lambda: ops.dense(x, w, act="silu"), lambda: ops.dense(x, w, checkpoint8=True),
+                 lambda: ops.gated_linear(x, w, w)):
+        for up in (dy, dy.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="no second derivatives"):
+                torch.autograd.grad(call(), x, up, create_graph=True)
+
+
 def test_calls_on_other_streams():
     ops = _ops()
     x, ws, bs, _, dy = _make(900, 130, 70, F32, 2)
