@@ -137,3 +137,15 @@ def test_modules():
     with pytest.raises(ValueError):
         ScaledEmbedding(4, 2, sparse=True)
     assert ScaledEmbedding(4, 2, padding_idx=1).padding_idx == 1
+
+
+def test_struct_layouts_match_header():
+    import os
+    import re
+
+    from conftest import ROOT
+    src = open(os.path.join(ROOT, "include", "aimx.h")).read()
+    for cname, py in (("AimxDense", _lib.Dense), ("AimxDenseGrad", _lib.DenseGrad)):
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{([^{}]*)\} %s;" % (cname, cname), src, re.S).group(1),
+                      flags=re.S)
+        assert re.findall(r"\**\s*(\w+)\s*(?:\[[^\]]*\])?\s*[;,]", body) == [f[0] for f in py._fields_]
