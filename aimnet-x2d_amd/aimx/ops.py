@@ -16,6 +16,7 @@ Beside the reference's own, for feed-forward stages on 32- and 16-bit tensors:
 """
 from __future__ import annotations
 
+import math
 import os
 
 import torch
@@ -1166,7 +1167,7 @@ def _matrix(what, name, t):
 
 class Packed8:
     """A tensor held in 8 bits (pack8): q int8 [M, Kq], exps int8 [M, Kq / 32], the shape and dtype it had.
-    nbytes is 33/32 of a byte per value (rows padded to 32)."""
+    Both parts contiguous and on the device for unpack8, which refuses others. nbytes is 33/32 of a byte per value (rows padded to 32)."""
     __slots__ = ("q", "exps", "shape", "dtype")
 
     def __init__(self, q, exps, shape, dtype):
@@ -1205,10 +1206,19 @@ def unpack8(packed, dtype=None):
     dtype = packed.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise _lib.AimxError(f"aimx.unpack8: fp32 or bf16, got {dtype}")
-    dev, K = packed.q.device, packed.shape[-1]
-    out = torch.empty(packed.shape, dtype=dtype, device=dev)
-    _launch(dev, "unpack8", _lib.load().aimx_unpack8, _DTYPES[dtype], ptr(packed.q), ptr(packed.exps),
-            packed.q.shape[0], K, ptr(out), K)
+    q, exps, shape = packed.q, packed.exps, packed.shape
+    # the kernel reads what the shape asks for
+    K = shape[-1] if len(shape) else 0
+    M, groups = math.prod(shape[:-1]), -(-K // PACK8_GROUP)
+    if K < 1 or q.dtype != torch.int8 or exps.dtype != torch.int8 or q.shape != (M, groups * PACK8_GROUP) or \
+            exps.shape != (M, groups) or not (q.is_contiguous() and exps.is_contiguous()) or q.device != exps.device:
+        raise _lib.AimxError(f"aimx.unpack8: a tensor {tuple(shape)} is held in contiguous int8 [{M}, "
+                             f"{groups * PACK8_GROUP}] and [{M}, {groups}] on one device, got {q.dtype} {tuple(q.shape)} "
+                             f"and {exps.dtype} {tuple(exps.shape)}")
+    _lib.require_device(q)
+    dev = q.device
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    _launch(dev, "unpack8", _lib.load().aimx_unpack8, _DTYPES[dtype], ptr(q), ptr(exps), M, K, ptr(out), K)
     return out
 
 

@@ -1,0 +1,58 @@
+"""What the feed-forward operators decide on the host, on CPU tensors with the launches recorded in place of run:
+which tensors reach a kernel, what is kept for a backward, and what is refused before a kernel could read memory that
+is not there."""
+import ctypes
+
+import pytest
+import torch
+
+from aimx import _lib, ops
+
+E = _lib.AimxError
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """[(what, C arguments)] of every call that would have been enqueued."""
+    seen = []
+    monkeypatch.setattr(_lib, "require_device", lambda *t: None)
+    monkeypatch.setattr(ops, "_launch", lambda device, what, fn, *args: seen.append((what, args)))
+    return seen
+
+
+def _packed(m=3, k=50, shape=None, q=None, exps=None):
+    kq = -(-k // 32) * 32
+    q = torch.zeros(m, kq, dtype=torch.int8) if q is None else q
+    exps = torch.zeros(m, kq // 32, dtype=torch.int8) if exps is None else exps
+    return ops.Packed8(q, exps, (m, k) if shape is None else shape, torch.float32)
+
+
+I8 = torch.int8
+
+
+@pytest.mark.parametrize("bad", [
+    dict(shape=(3, 70)), dict(shape=(4, 50)), dict(shape=(2, 50)), dict(shape=(3, 2, 50)), dict(shape=(150,)), dict(shape=()),
+    dict(shape=(3, 0)), dict(q=torch.zeros(3, 32, dtype=I8)), dict(q=torch.zeros(192, dtype=I8)), dict(q=torch.zeros(3, 64)),
+    dict(q=torch.zeros(64, 3, dtype=I8).t()), dict(q=torch.zeros(3, 128, dtype=I8)[:, :64]),
+    dict(exps=torch.zeros(3, 1, dtype=I8)), dict(exps=torch.zeros(2, 2, dtype=I8)), dict(exps=torch.zeros(3, 2)),
+    dict(exps=torch.zeros(3, 4, dtype=I8)[:, ::2]), dict(exps=torch.zeros(3, 2, dtype=I8, device="meta"))])
+def test_unpack8_refuses_parts_that_do_not_fit(bad, launches):
+    """The kernel reads as many bytes as the shape asks for: q and exps have to hold them."""
+    with pytest.raises(E, match="unpack8"):
+        ops.unpack8(_packed(**bad))
+    assert not launches
+
+
+def test_unpack8_takes_what_pack8_makes(launches):
+    assert ops.unpack8(_packed()).shape == (3, 50)
+    assert ops.unpack8(_packed(6, 50, (2, 3, 50))).shape == (2, 3, 50)
+    assert ops.unpack8(_packed(1, 50, (50,))).shape == (50,)
+    assert ops.unpack8(_packed(0, 50, (0, 4, 50))).shape == (0, 4, 50)
+    for shape in ((4, 33), (2, 0, 5), (7,)):
+        assert ops.unpack8(ops.pack8(torch.zeros(shape))).shape == shape
+
+
+def test_unpack8_refuses_host_memory():
+    """A form moved to the host (to offload it) is brought back by the caller: a kernel cannot read it there."""
+    with pytest.raises(E, match="HIP device"):
+        ops.unpack8(_packed())
