@@ -40,7 +40,7 @@ enum Act : int { ACT_NONE = -1, ACT_RELU = 0, ACT_LEAKYRELU = 1, ACT_ELU = 2, AC
 
 __device__ __forceinline__ float act_fwd(int kind, float v) {
   switch (kind) {
-    case ACT_RELU: return v > 0.f ? v : 0.f;
+    case ACT_RELU: return v <= 0.f ? 0.f : v;  // a NaN stays one
     case ACT_LEAKYRELU: return v > 0.f ? v : 0.01f * v;
     case ACT_ELU: return v > 0.f ? v : expm1f(v);
     case ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
@@ -54,7 +54,7 @@ __device__ __forceinline__ float act_fwd(int kind, float v) {
 // d act / d v evaluated at the pre-activation v (matches ATen's *_backward formulas).
 __device__ __forceinline__ float act_grad(int kind, float v) {
   switch (kind) {
-    case ACT_RELU: return v > 0.f ? 1.f : 0.f;
+    case ACT_RELU: return v <= 0.f ? 0.f : 1.f;
     case ACT_LEAKYRELU: return v > 0.f ? 1.f : 0.01f;
     case ACT_ELU: return v > 0.f ? 1.f : expf(v);
     case ACT_GELU: {

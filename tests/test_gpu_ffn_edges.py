@@ -1,0 +1,76 @@
+"""The feed-forward operators where values, layouts and modes are unusual: NaN and infinities in front of an
+activation, forward-mode derivatives, tracing, long row strides. Bounds as in tests/ffn_bounds.py."""
+import pytest
+import torch
+
+from ffn_bounds import act64, dact64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16 = torch.float32, torch.bfloat16
+ACTS = ["relu", "leakyrelu", "elu", "gelu", "silu"]
+
+
+def _ops():
+    from aimx import ops
+    return ops
+
+
+def _finite_or(a, b):
+    """NaN where b is NaN, the same infinities, finite elsewhere."""
+    a, b = a.detach().double().cpu(), b.double()
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isposinf(), b.isposinf()) and \
+        torch.equal(a.isneginf(), b.isneginf())
+
+
+# (70, 96, 40): at most 65536 values before the activation; (1100, 64, 200): more, N no multiple of 64
+SHAPES = [(70, 96, 40), (1100, 64, 200)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_nan_passes_every_activation(act, M, K, N, dtype):
+    """A row of x with a NaN gives a row of NaN, whatever the activation, in both products; no other row does."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(M, K, generator=g).to(dtype)
+    w, u = [(torch.randn(N, K, generator=g) * K ** -0.5).to(dtype).to(DEV) for _ in range(2)]
+    x[3, 5] = x[M - 1, K - 1] = float("nan")
+    hit = torch.zeros(M, dtype=torch.bool)
+    hit[[3, M - 1]] = True
+    xd = x.to(DEV)
+    for y in (ops.dense(xd, w, act=act), ops.dense(xd, w, act=act, residual=torch.ones(M, N, dtype=dtype, device=DEV)),
+              ops.gated_linear(xd, w, u, act=act)):
+        nan = y.isnan().cpu()
+        assert nan[hit].all() and not nan[~hit].any()
+    # a gate that is infinite, u of either sign: what the definition gives where the product itself is exact
+    if dtype == BF16:
+        x[3, 5], x[M - 1, K - 1] = float("inf"), -float("inf")
+        want = act64(act, x.double() @ w.cpu().double().t())
+        got = ops.dense(x.to(DEV), w, act=act)
+        # silu and gelu of -inf are 0 * inf, NaN by the formula: not asked for
+        fin = ~torch.isnan(want)
+        assert _finite_or(torch.where(fin, got.cpu(), 0), torch.where(fin, want, 0))
+
+
+def test_overflow_is_not_swallowed():
+    """An infinite fp32 activation may make NaN in the three-part product, and relu keeps the row from looking finite."""
+    ops = _ops()
+    x = torch.randn(40, 64, device=DEV)
+    x[7, 9] = float("inf")
+    w = torch.rand(30, 64, device=DEV) + 0.5  # every value of row 7 is infinite
+    for y in (ops.dense(x, w, act="relu"), ops.gated_linear(x, w, w, act="relu")):
+        assert not torch.isfinite(y[7]).any()
+        assert torch.isfinite(y[:7]).all() and torch.isfinite(y[8:]).all()
+
+
+def test_relu_of_nan_in_the_layer_products():
+    """The framework's own fp32 products use the same activation: nn.ReLU keeps a NaN too."""
+    ops = _ops()
+    x = torch.randn(70, 64, device=DEV)
+    x[3, 5] = float("nan")
+    w, b = torch.randn(48, 64, device=DEV), torch.randn(48, device=DEV)
+    y = ops.linear(x, w, b, act="relu")
+    want = torch.relu(x.cpu() @ w.cpu().t() + b.cpu())
+    assert torch.equal(y.isnan().cpu(), want.isnan()) and int(y.isnan().sum()) == 48
