@@ -467,6 +467,14 @@ __device__ __forceinline__ void epilogue(const Problem& p, floatx4 (&acc)[C::FN]
               out[0][e] = dd[e] * da[4 * i + e];
             }
           }
+          // Columns behind N only pad the rows. Their sums are x times zero, NaN where x is infinite, and 0 * NaN would
+          // reach dx, which reads them.
+          if (left < 4) {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) out[h][e] = e < left ? out[h][e] : 0.f;
+          }
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
             total[h][i] += out[h];

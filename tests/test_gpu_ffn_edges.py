@@ -74,3 +74,31 @@ def test_relu_of_nan_in_the_layer_products():
     y = ops.linear(x, w, b, act="relu")
     want = torch.relu(x.cpu() @ w.cpu().t() + b.cpu())
     assert torch.equal(y.isnan().cpu(), want.isnan()) and int(y.isnan().sum()) == 48
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("ckpt", [False, True])
+@pytest.mark.parametrize("act", ["relu", "leakyrelu", "elu"])
+def test_infinite_rows_keep_finite_gradients(act, ckpt, dtype):
+    """A row of x with an infinity: relu', leakyrelu' and elu' of plus and minus infinity are finite, and so is dx,
+    whatever N (columns that pad dP to 64 stay out of it). fp32's three-part product and the 8-bit form make NaN of
+    the row itself; every other row stays finite in each."""
+    ops = _ops()
+    for M, K, N in ((1100, 64, 200), (1100, 64, 192), (700, 72, 101), (70, 96, 40)):
+        g = torch.Generator().manual_seed(N)
+        x = torch.randn(M, K, generator=g).to(dtype)
+        w = (torch.randn(N, K, generator=g) * K ** -0.5).to(dtype)
+        w[w == 0] = 0.01
+        dy = torch.randn(M, N, generator=g).to(dtype)
+        x[3, 5] = float("inf")
+        xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        dx, dw = torch.autograd.grad(ops.dense(xd, wd, act=act, checkpoint8=ckpt), [xd, wd], dy.to(DEV))
+        rows = [i for i in range(M) if i != 3]
+        assert torch.isfinite(dx[rows]).all()
+        if dtype == BF16 and not ckpt:
+            assert torch.isfinite(dx).all(), (M, K, N)
+            p = x.double() @ w.double().t()
+            want = (dy.double() * dact64(act, p)) @ w.double()
+            # two roundings to bf16, of dP and of dx, and fp32 sums
+            mag = (dy.double() * dact64(act, p)).abs() @ w.double().abs()
+            assert ((dx.double().cpu() - want).abs() <= 2.0 ** -8 * (mag + want.abs()) * 1.01)[3].all()
