@@ -20,6 +20,7 @@ import math
 import os
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib
 from ._lib import ShellStack, ShellStackGrad, check, ptr, ptr_array, stream_ptr
@@ -1356,13 +1357,20 @@ def _dense_checks(what, x, ws, bs, act, res=None):
     return -1 if act is None else _lib.ACT_KIND[act]
 
 
+def _untracked():
+    """A call with no gradient asked for may go round its autograd Function: not inside
+    forward-mode differentiation, where the Function refuses dual inputs that the kernels would take without
+    their tangents."""
+    return _fwd._current_level < 0
+
+
 def _dense_apply(what, x, ws, bs, res, act, checkpoint8):
     grad = False
     if torch.is_grad_enabled():
         for t in (x, *ws, *bs, res):
             grad = grad or (t is not None and t.requires_grad)
-    if grad:
-        if x.numel() // x.shape[-1] > 1 << 22:
+    if grad or not _untracked():
+        if grad and x.numel() // x.shape[-1] > 1 << 22:
             raise _lib.AimxError(f"aimx.{what}: at most 2^22 rows where gradients are asked for")
         two = len(ws) == 2
         return _DenseFn.apply(x, ws[0], ws[1] if two else None, bs[0], bs[1] if two else None, res, act,
@@ -1449,6 +1457,6 @@ def embedding(index, table, scale=1.0, padding_idx=None):
     pad = -1 if padding_idx is None else int(padding_idx) % V
     _lib.require_device(table)
     index = (index if index.dtype == torch.int64 else index.long()).contiguous()
-    if torch.is_grad_enabled() and table.requires_grad:
+    if (torch.is_grad_enabled() and table.requires_grad) or not _untracked():
         return _Embedding.apply(index, table, float(scale), pad)
     return _embedding_forward(index, table.contiguous(), float(scale))

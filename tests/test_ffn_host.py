@@ -56,3 +56,23 @@ def test_unpack8_refuses_host_memory():
     """A form moved to the host (to offload it) is brought back by the caller: a kernel cannot read it there."""
     with pytest.raises(E, match="HIP device"):
         ops.unpack8(_packed())
+
+
+def _calls():
+    """One call of each differentiable operator, as a function of each of its tensors."""
+    x, w, b, r, t = torch.randn(4, 64), torch.randn(8, 64), torch.randn(8), torch.randn(4, 8), torch.randn(9, 16)
+    index = torch.tensor([1, 4])
+    return [(x, lambda v: ops.dense(v, w, b)), (w, lambda v: ops.dense(x, v)), (b, lambda v: ops.dense(x, w, v)),
+            (r, lambda v: ops.dense(x, w, residual=v, act="silu")), (x, lambda v: ops.gated_linear(v, w, w)),
+            (w, lambda v: ops.gated_linear(x, w, v, checkpoint8=True)), (t, lambda v: ops.embedding(index, v, 2.0))]
+
+
+def test_forward_mode_raises_instead_of_dropping_the_tangent(launches):
+    import torch.autograd.forward_ad as fw
+    for v, call in _calls():
+        with fw.dual_level():
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call(fw.make_dual(v, torch.ones_like(v)))
+            assert call(v) is not None  # no tangent: nothing to refuse
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (v,), (v,))

@@ -102,3 +102,22 @@ def test_infinite_rows_keep_finite_gradients(act, ckpt, dtype):
             # two roundings to bf16, of dP and of dx, and fp32 sums
             mag = (dy.double() * dact64(act, p)).abs() @ w.double().abs()
             assert ((dx.double().cpu() - want).abs() <= 2.0 ** -8 * (mag + want.abs()) * 1.01)[3].all()
+
+
+def test_forward_mode_is_refused():
+    """No tangent leaves these operators: a dual input raises, in whichever argument it stands, and plain inputs inside a
+    dual level work."""
+    import torch.autograd.forward_ad as fw
+    ops = _ops()
+    x, w, b = torch.randn(20, 32, device=DEV), torch.randn(24, 32, device=DEV), torch.randn(24, device=DEV)
+    index, table = torch.randint(0, 9, (12,), device=DEV), torch.randn(9, 16, device=DEV)
+    want = ops.dense(x, w, b, act="silu"), ops.gated_linear(x, w, w), ops.embedding(index, table)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.dense(dual(x), w, b), lambda: ops.dense(x, dual(w), b), lambda: ops.dense(x, w, dual(b)),
+                     lambda: ops.dense(x, w, b, residual=dual(want[0])), lambda: ops.gated_linear(x, w, dual(w)),
+                     lambda: ops.embedding(index, dual(table))):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call()
+        got = ops.dense(x, w, b, act="silu"), ops.gated_linear(x, w, w), ops.embedding(index, table)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
