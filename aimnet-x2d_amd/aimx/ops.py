@@ -1194,16 +1194,23 @@ def _pack8(what, x):
     return Packed8(q, exps, tuple(x.shape), x.dtype)
 
 
+def _no_trace(what):
+    if torch._C._is_tracing():
+        raise _lib.AimxError(f"aimx.{what}: not under torch.jit.trace (a trace cannot hold a Packed8)")
+
+
 def pack8(x):
     """The 8-bit form of a fp32 or bf16 tensor: groups of 32 values along the last dimension share a
     power-of-two scale 2^e, the least (from 2^-126) with 127 * 2^e >= max|x|; values are rounded to nearest
     even, so each comes back within 2^(e-1) <= max|x| / 127 of itself. A group with a NaN or an infinity comes
     back as NaN. Not differentiable (checkpoint8=True of dense and gated_linear is)."""
+    _no_trace("pack8")
     return _pack8("pack8", x.detach())
 
 
 def unpack8(packed, dtype=None):
     """The values a Packed8 stands for, in its own dtype or `dtype` (exact in both fp32 and bf16)."""
+    _no_trace("unpack8")
     dtype = packed.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise _lib.AimxError(f"aimx.unpack8: fp32 or bf16, got {dtype}")
@@ -1360,8 +1367,9 @@ def _dense_checks(what, x, ws, bs, act, res=None):
 def _untracked():
     """A call with no gradient asked for may go round its autograd Function: not inside
     forward-mode differentiation, where the Function refuses dual inputs that the kernels would take without
-    their tangents."""
-    return _fwd._current_level < 0
+    their tangents, nor under torch.jit.trace, which records the Function as a call but of a bare launch only the
+    allocation of its result."""
+    return _fwd._current_level < 0 and not torch._C._is_tracing()
 
 
 def _dense_apply(what, x, ws, bs, res, act, checkpoint8):

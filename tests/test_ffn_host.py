@@ -76,3 +76,18 @@ def test_forward_mode_raises_instead_of_dropping_the_tangent(launches):
             assert call(v) is not None  # no tangent: nothing to refuse
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (v,), (v,))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_traces_record_the_call(launches):
+    """torch.jit.trace holds the operator itself, not the allocation of its result."""
+    for v, call in _calls():
+        graph = str(torch.jit.trace(call, (v,), check_trace=False).graph)
+        assert ("^_DenseFn" in graph) != ("^_Embedding" in graph) and "aten::empty" not in graph
+    index = torch.tensor([1, 4])
+    assert "^_Embedding" in str(torch.jit.trace(lambda i: ops.embedding(i, torch.zeros(9, 16)), (index,),
+                                                check_trace=False).graph)
+    packed = ops.pack8(torch.zeros(4, 64))
+    for fn in (lambda v: ops.unpack8(ops.pack8(v)), lambda v: v + ops.unpack8(packed)):
+        with pytest.raises(E, match="torch.jit.trace"):
+            torch.jit.trace(fn, (torch.zeros(4, 64),), check_trace=False)

@@ -121,3 +121,17 @@ def test_forward_mode_is_refused():
                 call()
         got = ops.dense(x, w, b, act="silu"), ops.gated_linear(x, w, w), ops.embedding(index, table)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_traced_calls_run_again():
+    ops = _ops()
+    w, u, b = torch.randn(24, 32, device=DEV), torch.randn(24, 32, device=DEV), torch.randn(24, device=DEV)
+    table = torch.randn(9, 16, device=DEV)
+    for fn, make in ((lambda x: ops.dense(x, w, b, act="gelu"), lambda: torch.randn(20, 32, device=DEV)),
+                     (lambda x: ops.gated_linear(x, w, u), lambda: torch.randn(20, 32, device=DEV)),
+                     (lambda i: ops.embedding(i, table, 2.0), lambda: torch.randint(0, 9, (20,), device=DEV))):
+        traced = torch.jit.trace(fn, (make(),), check_trace=False)
+        for _ in range(3):
+            v = make()
+            assert torch.equal(traced(v), fn(v))
