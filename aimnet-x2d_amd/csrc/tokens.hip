@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void k_token_gather(const int64_t* __restrict_
     Cols<T> a;
     a.load(table + (ok ? v : 0) * D + c, ok ? D - c : 0);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) a.set(e, a.get(e) * scale);
+    for (int e = 0; e < kVec; ++e) a.set(e, ok ? a.get(e) * scale : 0.f);  // 0 * scale is NaN for an infinite scale
     a.store(out + i * D + c, D - c);
   }
 }

@@ -104,6 +104,16 @@ def test_infinite_rows_keep_finite_gradients(act, ckpt, dtype):
             assert ((dx.double().cpu() - want).abs() <= 2.0 ** -8 * (mag + want.abs()) * 1.01)[3].all()
 
 
+def test_lookup_out_of_range_is_zero_at_any_scale():
+    ops = _ops()
+    index = torch.tensor([0, 9, -1, 2], device=DEV)
+    for dtype in (F32, BF16):
+        table = torch.randn(4, 24, device=DEV).to(dtype)
+        for scale in (float("inf"), float("nan"), -2.0):
+            y = ops.embedding(index, table, scale)
+            assert (y[1] == 0).all() and (y[2] == 0).all()
+
+
 def test_forward_mode_is_refused():
     """No tangent leaves these operators: a dual input raises, in whichever argument it stands, and plain inputs inside a
     dual level work."""
