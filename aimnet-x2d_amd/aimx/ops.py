@@ -1158,11 +1158,15 @@ def _launch(device, what, fn, *args):
         return check(fn(*args, stream_ptr(device)), what)
 
 
-def _matrix(what, name, t):
-    """(t as [M, K] rows, row stride); t has unit column stride or is copied."""
+def _matrix(t):
+    """(t as [M, K] rows, row stride). Copied where the columns are apart or the rows further apart than the
+    products take (2^21 elements); the stride of a lone row says nothing."""
     t, ld = _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+    if t.shape[0] <= 1:
+        return t, t.shape[1]
     if ld > 1 << 21:
-        raise _lib.AimxError(f"aimx.{what}: {name} has a row stride over 2^21 elements")
+        t = t.contiguous()
+        ld = t.shape[1]
     return t, ld
 
 
@@ -1233,7 +1237,7 @@ def unpack8(packed, dtype=None):
 def _dense_struct(x2, ldx, ws, bs, act, prec):
     d = _lib.Dense()
     w = ws[0]
-    d.M, d.N, d.K = x2.shape[0], w.shape[0], w.shape[1]
+    d.M, d.N, d.K = 0 if x2 is None else x2.shape[0], w.shape[0], w.shape[1]
     d.halves, d.act, d.dtype, d.precision = len(ws), act, _DTYPES[w.dtype], prec
     d.x, d.ldx = ptr(x2), ldx
     d.ldw = w.shape[1]
@@ -1251,13 +1255,13 @@ def _dense_forward(x, ws, bs, res, act, prec, keep_pre):
     import ctypes
     lib = _lib.load()
     dev = x.device
-    x2, ldx = _matrix("dense", "x", x)
+    x2, ldx = _matrix(x)
     n = ws[0].shape[0]
     d = _dense_struct(x2, ldx, ws, bs, act, prec)
     y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
     d.y, d.ldy = ptr(y), n
     if res is not None:
-        r2, d.ldr = _matrix("dense", "residual", res)
+        r2, d.ldr = _matrix(res)
         d.res = ptr(r2)
     pre = None
     if keep_pre:
@@ -1308,12 +1312,13 @@ class _DenseFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dev = dy.device
         n, k = ws[0].shape
-        dy2, ldd = _matrix("dense", "dy", dy)
-        d = _dense_struct(kept, kept.stride(0), ws, bs, ctx.act, ctx.prec)
-        if exps is not None:
-            d.x, d.ldx, d.q, d.qexp = None, 0, ptr(kept), ptr(exps)
+        dy2, ldd = _matrix(dy)
+        if exps is None:
+            x2, ldx = _matrix(kept)
+            d = _dense_struct(x2, ldx, ws, bs, ctx.act, ctx.prec)
         else:
-            d.ldx = max(kept.stride(0), k)  # a single row's stride is whatever it is
+            d = _dense_struct(None, 0, ws, bs, ctx.act, ctx.prec)
+            d.M, d.q, d.qexp = kept.shape[0], ptr(kept), ptr(exps)
         d.pre = ptr(pre)
         g = _lib.DenseGrad()
         g.dy, g.ldd = ptr(dy2), ldd

@@ -91,3 +91,27 @@ def test_traces_record_the_call(launches):
     for fn in (lambda v: ops.unpack8(ops.pack8(v)), lambda v: v + ops.unpack8(packed)):
         with pytest.raises(E, match="torch.jit.trace"):
             torch.jit.trace(fn, (torch.zeros(4, 64),), check_trace=False)
+
+
+def test_long_row_strides_are_copied(launches):
+    """No layout of x, the residual or the incoming gradient is refused; what reaches the C entry keeps its limit."""
+    far = 2 ** 21 + 8
+
+    def rows(m, k):
+        return torch.empty_strided((m, k), (far, 1))
+
+    w, w2 = torch.randn(8, 16, requires_grad=True), torch.randn(8, 16)
+    for m in (1, 2, 3):
+        for x, r in ((rows(m, 16), None), (torch.randn(m, 16), rows(m, 8)), (rows(m, 16)[None], rows(m, 8)[None])):
+            launches.clear()
+            ys = [ops.dense(x, w, residual=r), ops.dense(x, w2, residual=r)] + ([ops.gated_linear(x, w, w)] if r is None else [])
+            for y in ys:
+                if y.requires_grad:
+                    torch.autograd.grad(y, w, rows(m, 8).view(y.shape))
+            kinds = [what for what, _ in launches]
+            assert kinds.count("dense_forward") == len(ys) and kinds.count("dense_backward") == len(ys) - 1
+            for what, args in launches:
+                d = args[0]._obj
+                assert d.M == m and 16 <= d.ldx <= 2 ** 21 and (not d.res or 8 <= d.ldr <= 2 ** 21)
+                if what == "dense_backward":
+                    assert 8 <= args[1]._obj.ldd <= 2 ** 21

@@ -145,3 +145,27 @@ def test_traced_calls_run_again():
         for _ in range(3):
             v = make()
             assert torch.equal(traced(v), fn(v))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_far_apart(dtype):
+    """Row strides over 2^21 elements are copied, in the inputs and in the gradient that autograd hands in."""
+    ops = _ops()
+    wide = torch.randn(3, 2 ** 21 + 72, device=DEV).to(dtype)
+    w, u = torch.randn(24, 40, device=DEV).to(dtype), torch.randn(24, 40, device=DEV).to(dtype)
+    r, dy, x = wide[:, 64:88], wide[:, 128:152], wide[:, 3:43]
+    assert x.stride(0) > 2 ** 21 and dy.stride(0) > 2 ** 21
+
+    def run(x, r, dy):
+        xs, ws, us, rs = [t.detach().requires_grad_() for t in (x, w, u, r)]
+        y = ops.dense(xs, ws, act="silu", residual=rs)
+        h = ops.gated_linear(xs, ws, us)
+        return [y, h, *torch.autograd.grad(y, [xs, ws, rs], dy), *torch.autograd.grad(h, [xs, ws, us], dy)]
+
+    for rows in (slice(0, 3), slice(1, 2)):
+        a, c, d = x[rows], r[rows], dy[rows]
+        assert all(torch.equal(p, q) for p, q in zip(run(a, c, d), run(a.clone(), c.clone(), d.clone())))
+    emb = torch.randn(5, 24, device=DEV).to(dtype).requires_grad_()
+    index = torch.tensor([1, 4, 1], device=DEV)
+    y = ops.embedding(index, emb)
+    assert torch.equal(torch.autograd.grad(y, emb, dy, retain_graph=True)[0], torch.autograd.grad(y, emb, dy.clone())[0])
