@@ -1291,6 +1291,8 @@ class _DenseFn(torch.autograd.Function):
         keep = x.dtype == _F32 and ctx.prec == PREC_FP32 and act >= 0 and not checkpoint8 and any(need[:5])
         y, pre, x2 = _dense_forward(x, ws, bs, res, act, ctx.prec, keep)
         ctx.act, ctx.shape, ctx.halves = act, x.shape, len(ws)
+        if not any(need[:5]):  # the residual's gradient is dy
+            return y
         kept, exps = x2, None
         if checkpoint8:
             p = _pack8("dense", x2)
@@ -1306,10 +1308,12 @@ class _DenseFn(torch.autograd.Function):
         # requires grad); an edge to x would keep alive what checkpoint8 frees.
         if torch.is_grad_enabled():
             raise _lib.AimxError("aimx.dense, gated_linear: no second derivatives (backward with create_graph=True)")
+        need = ctx.needs_input_grad
+        if not any(need[:5]):
+            return None, None, None, None, None, dy if need[5] else None, None, None
         lib = _lib.load()
         kept, exps, pre, *rest = ctx.saved_tensors
         ws, bs = rest[:ctx.halves], rest[ctx.halves:]
-        need = ctx.needs_input_grad
         dev = dy.device
         n, k = ws[0].shape
         dy2, ldd = _matrix(dy)
@@ -1334,12 +1338,11 @@ class _DenseFn(torch.autograd.Function):
             db = [torch.empty(n, dtype=dy.dtype, device=dev) for _ in ws]
             for i, t in enumerate(db):
                 g.db[i] = ptr(t)
-        if dx is not None or dw is not None or db is not None:
-            args = ctypes.byref(d), ctypes.byref(g)
-            g.workspace_bytes = lib.aimx_dense_backward_workspace_bytes(*args)
-            work = _workspace(g.workspace_bytes, dev)
-            g.workspace = ptr(work)
-            _launch(dev, "dense_backward", lib.aimx_dense_backward, *args)
+        args = ctypes.byref(d), ctypes.byref(g)
+        g.workspace_bytes = lib.aimx_dense_backward_workspace_bytes(*args)
+        work = _workspace(g.workspace_bytes, dev)
+        g.workspace = ptr(work)
+        _launch(dev, "dense_backward", lib.aimx_dense_backward, *args)
         at = lambda v, i: v[i] if v is not None and i < len(v) and need[i + (1 if v is dw else 3)] else None  # noqa: E731
         return dx, at(dw, 0), at(dw, 1), at(db, 0), at(db, 1), dy if need[5] else None, None, None
 
@@ -1383,7 +1386,8 @@ def _dense_apply(what, x, ws, bs, res, act, checkpoint8):
         for t in (x, *ws, *bs, res):
             grad = grad or (t is not None and t.requires_grad)
     if grad or not _untracked():
-        if grad and x.numel() // x.shape[-1] > 1 << 22:
+        if x.numel() // x.shape[-1] > 1 << 22 and torch.is_grad_enabled() and \
+                any(t is not None and t.requires_grad for t in (x, *ws, *bs)):
             raise _lib.AimxError(f"aimx.{what}: at most 2^22 rows where gradients are asked for")
         two = len(ws) == 2
         return _DenseFn.apply(x, ws[0], ws[1] if two else None, bs[0], bs[1] if two else None, res, act,

@@ -115,3 +115,22 @@ def test_long_row_strides_are_copied(launches):
                 assert d.M == m and 16 <= d.ldx <= 2 ** 21 and (not d.res or 8 <= d.ldr <= 2 ** 21)
                 if what == "dense_backward":
                     assert 8 <= args[1]._obj.ldd <= 2 ** 21
+
+
+def test_a_residual_alone_keeps_nothing(launches):
+    """The residual's gradient is the incoming one: no input is kept for it, packed or held to the rows of a backward."""
+    x, w, r = torch.randn(4, 64), torch.randn(8, 64), torch.randn(4, 8, requires_grad=True)
+    dy = torch.randn(4, 8)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        for kw in (dict(act="silu"), dict(checkpoint8=True)):
+            assert torch.equal(torch.autograd.grad(ops.dense(x, w, residual=r, **kw), r, dy)[0], dy)
+    assert not kept and [what for what, _ in launches] == ["dense_forward"] * 2
+    many = torch.empty(1, dtype=torch.bfloat16).expand(2 ** 22 + 1, 1)
+    ops.dense(many, many[:1], residual=torch.empty(1, dtype=torch.bfloat16, requires_grad=True).expand(2 ** 22 + 1, 1))
+    with pytest.raises(E, match="2\\^22 rows"):
+        ops.dense(many, torch.empty(1, 1, dtype=torch.bfloat16, requires_grad=True))
+    # beside other gradients it is still dy
+    ws = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.dense(x, ws, residual=r), [ws, r], dy)[1], dy)
+    assert launches[-1][0] == "dense_backward"
