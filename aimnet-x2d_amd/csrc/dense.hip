@@ -403,7 +403,7 @@ void backward(Ctx& c, Carve& ws, const AimxDense* d, const AimxDenseGrad* g) {
     parts = cdiv(M, kDpreRows);
     if (has_db) sums = a.sums = ws.take<float>(parts * H * N);
     if (!c.dry && !c.rc && M > 0 && (a.rows || a.sums)) {
-      if (Np / 64 * parts > INT32_MAX) c.rc = AIMX_EARG;
+      if (!grid_ok(Np / 64 * parts, 256)) c.rc = AIMX_EARG;
       else if (!k.fp32 && fine) dpre_go<uint16_t, 3>(c, a, (int)H);
       else if (!k.fp32) dpre_go<uint16_t, 1>(c, a, (int)H);
       else if (k.planes == 3) dpre_go<float, 3>(c, a, (int)H);

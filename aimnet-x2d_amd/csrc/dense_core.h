@@ -716,12 +716,15 @@ Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split, bool fp32
 int launch_one(const Problem& p, int tile, int epi, int across, bool fp32, hipStream_t st);
 int launch_split(const Problem& p, int tile, int pa, int pb, int epi, int across, bool fp32, hipStream_t st);
 
+// a dispatch counts its work items of a dimension in 32 bits
+inline bool grid_ok(int64_t blocks, int64_t threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
+
 template <typename C, int EPI, int ACROSS, typename T>
 int launch_config(const Problem& p, hipStream_t st) {
   constexpr int TC = C::TN / (EPI == kGated || EPI == kGatedGrad ? 2 : 1);
   // the backward epilogues write the padding behind column N too
   const int64_t tm = cdiv(p.M, C::TM), tn = cdiv(EPI == kDenseGrad || EPI == kGatedGrad ? p.np : p.N, TC);
-  if (tm * tn > (int64_t)INT32_MAX) return AIMX_EARG;
+  if (!grid_ok(tm * tn, C::kThreads)) return AIMX_EARG;
   hipLaunchKernelGGL((k_dense<C, EPI, ACROSS, T>), dim3((unsigned)(tm * tn), (unsigned)p.splits), dim3(C::kThreads), 0,
                      st, p, (int)tm, (int)tn);
   AIMX_CHECK_LAUNCH();

@@ -134,3 +134,18 @@ def test_a_residual_alone_keeps_nothing(launches):
     ws = w.clone().requires_grad_()
     assert torch.equal(torch.autograd.grad(ops.dense(x, ws, residual=r), [ws, r], dy)[1], dy)
     assert launches[-1][0] == "dense_backward"
+
+
+def test_c_products_refuse_more_work_items_than_a_dispatch_counts():
+    """2^32 work items in a dimension: refused here, before the launch, not left to the runtime."""
+    lib = _lib.load()
+    d = _lib.Dense()
+    d.M, d.N, d.K, d.halves, d.act, d.dtype = 2 ** 36, 64, 64, 1, -1, 1
+    d.x, d.ldx, d.w[0], d.ldw, d.y, d.ldy = 4096, 64, 8192, 64, 16384, 64
+    assert lib.aimx_dense_workspace_bytes(ctypes.byref(d)) == 0  # read in place: the product is the first launch
+    assert lib.aimx_dense_forward(ctypes.byref(d), None) == -1
+    d.M, d.N, d.K, d.dtype = 2 ** 22, 2 ** 21, 2 ** 21, 0  # db alone: the column sums of dy
+    d.ldx = d.ldw = d.ldy = 2 ** 21
+    g = _lib.DenseGrad()
+    g.dy, g.ldd, g.db[0], g.workspace, g.workspace_bytes = 4096, 2 ** 21, 8192, 1 << 20, 1 << 62
+    assert lib.aimx_dense_backward(ctypes.byref(d), ctypes.byref(g), None) == -1
