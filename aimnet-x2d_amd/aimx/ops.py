@@ -1206,8 +1206,9 @@ def _no_trace(what):
 def pack8(x):
     """The 8-bit form of a fp32 or bf16 tensor: groups of 32 values along the last dimension share a
     power-of-two scale 2^e, the least (from 2^-126) with 127 * 2^e >= max|x|; values are rounded to nearest
-    even, so each comes back within 2^(e-1) <= max|x| / 127 of itself. A group with a NaN or an infinity comes
-    back as NaN. Not differentiable (checkpoint8=True of dense and gated_linear is)."""
+    even, so each comes back within 2^(e-1) of itself: within max|x| / 127, or 2^-127 where that is more. Groups
+    with max|x| > 127 * 2^121 = 3.376e38 are kept below overflow, their values within 2^122. A group with a NaN
+    or an infinity comes back as NaN. Not differentiable (checkpoint8=True of dense and gated_linear is)."""
     _no_trace("pack8")
     return _pack8("pack8", x.detach())
 

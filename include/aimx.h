@@ -636,7 +636,8 @@ int aimx_dense_backward(const AimxDense* d, const AimxDenseGrad* g, aimx_stream_
  * 2^e, e the least integer >= -126 with 127 * 2^e >= max|x| of the group; q = round-to-even(x / 2^e).
  * q [M, Kq] int8 (8-byte aligned, zeros behind column K), exps [M, Kq / 32] int8, Kq = K rounded up to 32.
  * A group with a NaN or an infinity has e = 127 and unpacks as NaN. q * 2^e is exactly a bf16. The largest
- * fp32 values (e = 122) are kept below overflow (|q| <= 63).
+ * values (e = 122, a group's largest above 127 * 2^121) are kept below overflow (|q| <= 63). A value comes back within
+ * 2^(e-1), which is at most max|x| / 127 unless e = -126, where it is 2^-127; with e = 122 within 2^122.
  * ------------------------------------------------------------------------------------------ */
 int aimx_pack8(int32_t dtype, const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* q, int8_t* exps,
                aimx_stream_t stream);

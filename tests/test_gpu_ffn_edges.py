@@ -169,3 +169,23 @@ def test_rows_far_apart(dtype):
     index = torch.tensor([1, 4, 1], device=DEV)
     y = ops.embedding(index, emb)
     assert torch.equal(torch.autograd.grad(y, emb, dy, retain_graph=True)[0], torch.autograd.grad(y, emb, dy.clone())[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_pack8_error_bound(dtype):
+    """Values come back within max(top / 127, 2^-127) of themselves, top the group's largest; within 2^122 where top is
+    above 127 * 2^121. Both ends pass top / 127 alone: 2^-128 comes back as 0, the largest floats 2^122 off."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(2)
+    tops = torch.exp2(torch.cat([torch.linspace(-149, -100, 99), torch.linspace(-99, 127.99, 500),
+                                 torch.linspace(127.9, 127.999, 30)]).double()).float().to(dtype)
+    x = (torch.rand(len(tops), 32, generator=g, dtype=torch.float64) * 2 - 1).mul_(tops.double()[:, None]).to(dtype)
+    x[:, 3] = tops
+    x = torch.where(torch.isfinite(x), x, torch.zeros_like(x))
+    v, top = x.double(), x.double().abs().amax(1, keepdim=True)
+    err = (ops.unpack8(ops.pack8(x.to(DEV))).double().cpu() - v).abs()
+    bound = torch.where(top > 127 * 2.0 ** 121, torch.full_like(top, 2.0 ** 122), (top / 127).clamp(min=2.0 ** -127))
+    assert (err <= bound).all()
+    past = (err > top / 127).any(1)
+    assert past[top[:, 0] < 2.0 ** -127].any() and past[top[:, 0] > 127 * 2.0 ** 121].any()
+    assert not past[(top[:, 0] > 2.0 ** -120) & (top[:, 0] <= 127 * 2.0 ** 121)].any()
