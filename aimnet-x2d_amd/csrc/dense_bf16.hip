@@ -15,8 +15,8 @@ using Small = Config<1, 1, 64, 64, 2, 2, 64>;     // 4 waves of 32 x 32, 32 KB: 
 // 20480 x 2048 (K = 512) three rounds of large tiles take 80 us and five of middle ones 68.
 Plan plan_one(int64_t M, int64_t columns, int64_t K, bool may_split) {
   static const Shape shapes[] = {{0, 256, 256, 64, 1, 1.74, 9.}, {1, 128, 128, 64, 2, 1.08, 4.5}, {2, 64, 64, 64, 5, 0.85, 3.}};
-  const int64_t force = tune_i64("AIMX_DENSE_TILE", -1);
-  if (force >= 0) return pick(shapes + force, 1, M, columns, K, may_split);
+  const int64_t force = opt_i64("AIMX_DENSE_TILE", -1);  // test hook (aimx_set_option)
+  if (force >= 0 && force < 3) return pick(shapes + force, 1, M, columns, K, may_split);
   return pick(shapes, 3, M, columns, K, may_split);
 }
 

@@ -45,8 +45,8 @@ int go(const Problem& p, int pa, int pb, int epi, int across, hipStream_t st) {
 Plan plan_split(int64_t M, int64_t columns, int64_t K, bool may_split, bool fp32) {
   static const Shape shapes[] = {{0, 128, 128, 32, 1, 1.1, 9.}, {1, 64, 64, 32, 3, 1.5, 4.}, {2, 256, 128, 32, 1, 1.95, 12.}};
   if (!fp32) return pick(shapes + 1, 1, M, columns, K, may_split);
-  const int64_t force = tune_i64("AIMX_DENSE_SPLIT_TILE", -1);
-  if (force >= 0) return pick(shapes + force, 1, M, columns, K, may_split);
+  const int64_t force = opt_i64("AIMX_DENSE_SPLIT_TILE", -1);  // test hook (aimx_set_option)
+  if (force >= 0 && force < 3) return pick(shapes + force, 1, M, columns, K, may_split);
   return pick(shapes, 3, M, columns, K, may_split);
 }
 

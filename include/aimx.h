@@ -50,6 +50,9 @@ const char* aimx_version(void);
  *   "AIMX_WGRAD_BB"     64 / 80 = weight-gradient block edge
  *   "AIMX_GEMM_DEEP"    0 = few-row deep-K products on the LDS-staged tiles; 8 = 8 waves
  *   "AIMX_HOP_MAX_ROWS" n = the hop's row-range splitting at n rows per launch (not 2^31)
+ *   "AIMX_DENSE_TILE"   0 / 1 / 2 = dense and gated products of one bf16 plane a side on 256 x 256 / 128 x 128 /
+ *                       64 x 64 tiles
+ *   "AIMX_DENSE_SPLIT_TILE" 0 / 1 / 2 = those of fp32 tensors at fp32 accuracy on 128 x 128 / 64 x 64 / 256 x 128 tiles
  * The tuning build (make tune -> lib/libaimx_tune.so) also reads these names, and its A/B knobs
  * (tune_i64 in csrc: variants measured slower, kept for re-measurement), from the environment; the
  * product library compiles those knobs to their defaults. aimx_set_option returns AIMX_EARG for a
