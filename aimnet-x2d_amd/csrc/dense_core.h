@@ -2,7 +2,8 @@
 // with the epilogues of the dense and gated operators.
 //
 // Operands are bf16 "planes": a bf16 matrix is one plane, an fp32 matrix three whose sum is the matrix,
-// x = x1 + x2 + x3 exactly (8 + 8 + 8 mantissa bits). The product of two three-plane
+// x = x1 + x2 + x3 exactly (8 + 8 + 8 mantissa bits) from 2^-110 on; below, where the third plane's last bit would
+// be less than bf16's least subnormal 2^-133, within 2^-134. The product of two three-plane
 // operands takes the six plane products x_i w_j with i + j <= 4 (Henry, Tang, Heinecke, "Leveraging the
 // bfloat16 Artificial Intelligence Datatype For Higher-Precision Computations", 2019): what is left out
 // is at most 2^-23 |x||w|, the products of planes are exact (8 x 8 bits) and their sums are
@@ -49,7 +50,7 @@ __device__ __forceinline__ uint16_t to_bf16(float v) {
 __device__ __forceinline__ float from_bf16(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
 
 // The three planes of v, each the nearest bf16 of what is left: |x2| <= 2^-8 |x|, |x3| <= 2^-16 |x|, and the
-// third is exact (24 = 8 + 8 + 8 bits). A NaN or infinity goes whole into the first plane; what it then
+// third is exact (24 = 8 + 8 + 8 bits; |x| >= 2^-110). A NaN or infinity goes whole into the first plane; what it then
 // multiplies in the other operand's lower planes may be zero, so an infinite operand can make a NaN
 // where the one-plane product has an infinity.
 __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {

@@ -590,7 +590,7 @@ int aimx_pad_batch(const AimxPadBatch* p, aimx_stream_t stream);
  * x [M, K] (row stride ldx), each w [N, K] (row stride ldw), each b [N], res and y [M, N]: all of `dtype`.
  * precision: of fp32 tensors. AIMX_PREC_FP32: fp32 accuracy on the bf16 matrix cores (three exact bf16
  * parts per operand, six products); AIMX_PREC_BF16: operands rounded to bf16, everything else fp32.
- * Sums are fp32. An infinite operand of an AIMX_PREC_FP32 product may give NaN instead of an infinity.
+ * Sums are fp32. AIMX_PREC_FP32 reads operand values below 2^-110 within 2^-134. An infinite operand of an AIMX_PREC_FP32 product may give NaN instead of an infinity.
  * pre (nullable, fp32 [M, halves, N rounded up to 8], 16-byte aligned): the values before the activation, kept for
  * aimx_dense_backward; without them (act != none) the backward computes them again from x or its 8-bit
  * form, which bf16 tensors do faster. An fp32 product (AIMX_PREC_FP32) from x itself keeps them: there

@@ -189,3 +189,36 @@ def test_pack8_error_bound(dtype):
     past = (err > top / 127).any(1)
     assert past[top[:, 0] < 2.0 ** -127].any() and past[top[:, 0] > 127 * 2.0 ** 121].any()
     assert not past[(top[:, 0] > 2.0 ** -120) & (top[:, 0] <= 127 * 2.0 ** 121)].any()
+
+
+@pytest.mark.parametrize("low,high", [(-110, -60), (-140, -110)])
+def test_small_magnitudes_fp32(low, high):
+    """Three bf16 parts are an fp32 value down to 2^-110, where the last bit of the third is bf16's least subnormal
+    2^-133; below, their sum is off by at most half of that. Either operand of the forward product and of both
+    gradient products small, the other around 2^30."""
+    g = torch.Generator().manual_seed(-low)
+
+    def small(*s):
+        v = (torch.rand(*s, generator=g) + 1) * torch.exp2(torch.randint(low, high, s, generator=g).float())
+        return torch.where(torch.rand(*s, generator=g) < 0.5, v, -v)
+
+    lost = 2.0 ** -134 if low < -110 else 0.0
+    ops = _ops()
+    for M, K, N in ((40, 96, 50), (130, 200, 70)):
+        large = lambda *s: torch.randn(*s, generator=g) * 2.0 ** 30  # noqa: E731
+
+        def check(got, a, b):  # got = a b^T, a small
+            a, b = a.double(), b.double()
+            bound = ((a.shape[1] + 16) * 2.0 ** -24 * a.abs() + lost) @ b.t().abs() + 2.0 ** -24 * (a @ b.t()).abs()
+            assert ((got.double().cpu() - a @ b.t()).abs() <= bound).all(), (M, K, N)
+
+        x, w = small(M, K), large(N, K)
+        check(ops.dense(x.to(DEV), w.to(DEV)), x, w)
+        check(ops.dense(w.to(DEV), x.to(DEV)).t(), x, w)  # the small operand as the weight
+        dy, x = small(M, N), large(M, K)
+        xs, ws = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        dx, dw = torch.autograd.grad(ops.dense(xs, ws), [xs, ws], dy.to(DEV))
+        check(dx, dy, w.t())
+        check(dw, dy.t(), x.t())
+        dx, dw = torch.autograd.grad(ops.dense(xs, ws, checkpoint8=True), [xs, ws], dy.to(DEV))
+        check(dx, dy, w.t())
