@@ -597,7 +597,8 @@ int aimx_pad_batch(const AimxPadBatch* p, aimx_stream_t stream);
  * pre must not be NULL in the backward.
  * The workspace (16-byte aligned, aimx_dense_workspace_bytes / aimx_dense_backward_workspace_bytes) holds
  * staged operands and partial sums. Sums over ranges of k and of rows are joined in a fixed order.
- * Row strides <= 2^21 elements, N, K <= 2^21; the backward takes M <= 2^22 rows.
+ * Row strides <= 2^21 elements, N, K <= 2^21; the backward takes M <= 2^22 rows (dw and db are fp32 sums over them, off
+ * by at most M 2^-24 of the magnitudes).
  *
  * aimx_dense_backward: dy [M, N] -> dx [M, K], dw [N, K] (contiguous), db [N], each written when its
  * pointer is given (dw and db of both halves or of neither). It reads x, w, pre of d (b only where pre is
