@@ -20,8 +20,8 @@
 // Bound: the matrix cores, then LDS reads (a 128 x 64 wave tile reads 12 KB per 32 matrix instructions, three
 // quarters of LDS's rate; a 64 x 64 one all of it), then the epilogue where k is short. Measured, us and TFLOP/s of a
 // launch: 32768 x 1024 over k = 8192 (dx) 450, 1220; 8192 x 1024 over k = 32768 (dW) 452, 1215; the gated forward
-// 32768 x 1024 -> 2 x 4096 538, 1022, its gradient epilogue 695; 20480 x 512 -> 2 x 2048 110, 780. Three planes
-// a side, as fp32: 32768 x 2048 over k = 1024 626, 218.
+// 32768 x 1024 -> 2 x 4096 538, 1022, its gradient epilogue 695; 20480 x 512 -> 2 x 2048 113, 760. Three planes
+// a side, as fp32: 32768 x 2048 over k = 1024 639 to 656, 209 to 215.
 #pragma once
 
 #include <algorithm>
