@@ -1172,7 +1172,8 @@ def _matrix(t):
 
 class Packed8:
     """A tensor held in 8 bits (pack8): q int8 [M, Kq], exps int8 [M, Kq / 32], the shape and dtype it had.
-    Both parts contiguous and on the device for unpack8, which refuses others. nbytes is 33/32 of a byte per value (rows padded to 32)."""
+    unpack8 takes both parts contiguous and on the device, and refuses others. nbytes is 33/32 of a byte per value
+    (rows padded to 32)."""
     __slots__ = ("q", "exps", "shape", "dtype")
 
     def __init__(self, q, exps, shape, dtype):
